@@ -439,6 +439,148 @@ rtenhip_status rtenhip_sharded_run_host(rtenhip_sharded* s, const rtenhip_tensor
  * zero-padded), for a device-resident consumer; NULL otherwise. */
 const float* rtenhip_sharded_gathered(rtenhip_sharded* s, int32_t shard);
 
+/* ---- decoder operators ---------------------------------------------------
+ * What a decoder that answers token by token needs next to the operators
+ * above: the norm and rotation of queries and keys, attention over a paged
+ * cache, and sampling.  RTen has no counterparts; results are those of the
+ * formulas given here, computed in 32 bits or more.  The calls neither
+ * allocate nor synchronize, keep nothing between calls (workspaces are the
+ * caller's, so two captured graphs share one only if their caller says so)
+ * and can be captured.  Tensors live on the context's device. */
+
+/* Element type of a cache. */
+typedef enum {
+  RTENHIP_CACHE_F32 = 0,
+  RTENHIP_CACHE_F16 = 1,
+  RTENHIP_CACHE_BF16 = 2,
+} rtenhip_cache_dtype;
+
+/* Keys and values of past tokens in pages of page_size tokens.  Row (page,
+ * slot, head) of head_dim contiguous elements starts at
+ * page * strides[0] + slot * strides[1] + head * strides[2] (elements).
+ * head_dim is a multiple of 8, at most 256; every row starts on 16 bytes;
+ * page_size is any number from 1 to 65536. */
+typedef struct {
+  void* k;
+  void* v;
+  int32_t dtype;                     /* rtenhip_cache_dtype */
+  int32_t page_size;
+  int64_t n_pages;
+  int32_t n_heads;
+  int32_t head_dim;
+  int64_t k_strides[3];
+  int64_t v_strides[3];
+} rtenhip_kv_cache;
+
+/* The sequences of a call.  Sequence s has the new tokens q_starts[s] ..
+ * q_starts[s + 1] - 1 of the call's rows (q_starts NULL: row s alone, one row
+ * per sequence) and kv_lens[s] cached tokens, its new ones being the last of
+ * them: new token i has position kv_lens[s] - (new tokens of s) + i.  Token j
+ * is in slot j % page_size of page page_table[s * table_stride + j /
+ * page_size]; an entry outside [0, n_pages), such as -1, is no page: nothing
+ * is written to it and its tokens are seen by nobody.  q_starts does not
+ * decrease; rows from q_starts[n_seqs] on are padding, not read or written.
+ * A sequence may have no new tokens or no cached ones.  All device arrays. */
+typedef struct {
+  const int32_t* page_table;         /* [n_seqs][max_pages] */
+  int64_t table_stride;
+  const int32_t* kv_lens;            /* [n_seqs] */
+  const int32_t* q_starts;           /* [n_seqs + 1] or NULL */
+  int32_t n_seqs;
+  int32_t max_pages;
+} rtenhip_sequences;
+
+/* Norm and rotation of head rows x of head_dim values:
+ *   y = x / sqrt(mean(x * x) + epsilon) * scale     (scale NULL: y = x)
+ *   the pairs (y[i], y[i + R/2]) -- interleaved: (y[2i], y[2i+1]) -- for
+ *   i < R/2, R = rotary_dim, turn by positions[t] * inv_freq[i] (the angle
+ *   formed and reduced in 64 bits): (a cos - b sin, b cos + a sin);
+ *   y[R..] stays.
+ * R is a multiple of 8 from 0 to head_dim.  All device arrays, on 4 bytes. */
+typedef struct {
+  const float* q_scale;              /* [head_dim] or NULL: no norm of q */
+  const float* k_scale;              /* [head_dim] or NULL: no norm of k */
+  const float* inv_freq;             /* [rotary_dim / 2] */
+  const int32_t* positions;          /* [tokens] */
+  float epsilon;
+  int32_t rotary_dim;
+  int32_t interleaved;
+} rtenhip_rotary;
+
+/* q [tokens, q heads, head_dim] and k [tokens, k heads, head_dim] into q_out
+ * and k_out (each may be its input; otherwise they share no memory with the
+ * inputs).  Rows: unit stride along head_dim, starts on 16 bytes, any token
+ * and head strides (views into a fused projection's output). */
+rtenhip_status rtenhip_qk_norm_rotary_f32(rtenhip_ctx* ctx, const rtenhip_tensor* q,
+                                          const rtenhip_tensor* k, const rtenhip_rotary* r,
+                                          rtenhip_tensor* q_out, rtenhip_tensor* k_out);
+/* The same with k's rows and v [tokens, k heads, head_dim] written into the
+ * sequences' cache (rounded to nearest even in a 16-bit cache, past its
+ * range to infinity), q's into q_out.  r->positions NULL: the position in the
+ * sequence; given, it turns the rows but does not move their slots.  Two
+ * sequences of a call must not share a page that one of them writes. */
+rtenhip_status rtenhip_qk_norm_rotary_append_f32(rtenhip_ctx* ctx, const rtenhip_tensor* q,
+                                                 const rtenhip_tensor* k, const rtenhip_tensor* v,
+                                                 const rtenhip_rotary* r,
+                                                 const rtenhip_kv_cache* cache,
+                                                 const rtenhip_sequences* seqs,
+                                                 rtenhip_tensor* q_out);
+
+/* Attention of the call's new tokens over their sequences' cached ones.  q
+ * and out [tokens, q heads, head_dim] (rows as above); query head h reads
+ * cache head h / (q heads / n_heads).  The token at position p sees token j
+ * if 0 <= j <= p, j has a page, and window == 0, or j > p - window, or
+ * j < sinks:
+ *   out = sum_j softmax_j(scale * q . k_j) v_j,  zeros if it sees none.
+ * Products of a 16-bit or f32 cache are formed to about 22 bits and summed in
+ * 32.  Slots that no query of the call sees are read but have no effect,
+ * whatever they hold; a NaN or an infinity in a key or value leaves the
+ * queries that do not see its token as they are (the output of those that do
+ * is undefined).  out may be q.  workspace: at least
+ * rtenhip_paged_attention_workspace() bytes, on 16 bytes, contents of no
+ * meaning before or after; calls that may run at the same time need one each. */
+rtenhip_status rtenhip_paged_attention_workspace(const rtenhip_tensor* q,
+                                                 const rtenhip_kv_cache* cache,
+                                                 const rtenhip_sequences* seqs, size_t* bytes);
+rtenhip_status rtenhip_paged_attention_f32(rtenhip_ctx* ctx, const rtenhip_tensor* q,
+                                           const rtenhip_kv_cache* cache,
+                                           const rtenhip_sequences* seqs, float scale,
+                                           int32_t window, int32_t sinks, void* workspace,
+                                           size_t workspace_bytes, rtenhip_tensor* out);
+
+/* Filters of rtenhip_sample_f32: one value for all rows, or one per row from
+ * the device array beside it where that is not NULL. */
+typedef struct {
+  float temperature, top_p, min_p;
+  int32_t top_k;
+  const float* temperatures;         /* [rows] or NULL */
+  const float* top_ps;
+  const float* min_ps;
+  const int32_t* top_ks;
+} rtenhip_sampling;
+
+/* One token for each row of logits [rows, vocab] (unit stride along vocab).
+ * With l the row, max its largest value and T the temperature, token i weighs
+ * m_i = exp((l_i - max) / T) (64 bits).  In the order of falling l, equal
+ * ones by rising index:
+ *   top-k keeps the first k (k <= 0: all);
+ *   top-p then keeps the tokens that the kept mass before them is less than
+ *     p * (all kept mass) of, the first one always (p >= 1: all);
+ *   min-p then keeps those with m_i >= min_p (min_p <= 0: all; the first
+ *     one always).
+ * The token is the lowest index at which the kept mass up to it, in the order
+ * of the indices, exceeds u * (all kept mass), u = uniforms[row] in [0, 1)
+ * (brought into that range); logprobs[row] (NULL: not wanted) is the log of
+ * its share of the kept mass.  T <= 0 or NaN: the largest l, the first of
+ * equals, log 0.  NaN counts as -infinity and is never taken; of +infinities
+ * each weighs 1 and the rest 0; a row of nothing else gives -1 and -infinity.
+ * vocab from 1 to 2^24.  workspace as for rtenhip_paged_attention_f32. */
+rtenhip_status rtenhip_sample_workspace(int64_t rows, int64_t vocab, size_t* bytes);
+rtenhip_status rtenhip_sample_f32(rtenhip_ctx* ctx, const rtenhip_tensor* logits,
+                                  const rtenhip_sampling* sampling, const float* uniforms,
+                                  void* workspace, size_t workspace_bytes, int32_t* tokens,
+                                  float* logprobs);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,78 @@
+// Shared parts of the decoder operators (rotary.hip, paged_attention.hip,
+// sampling.hip): the paged cache and the sequences of a call as the kernels
+// see them, and the checks of their C descriptors.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "common.h"
+#include "ctx.h"
+#include "fastdiv_dev.h"
+
+namespace rtenhip {
+
+// A paged cache for the kernels: element strides, any order of page, slot and
+// head, head_dim contiguous elements per row.
+struct CacheView {
+  char *k, *v;
+  int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;
+  int64_t n_pages;
+  FastDiv page_div;
+  int page_size, heads, dim;
+};
+
+struct SeqView {
+  const int* table;     // [n][max_pages], row stride table_stride
+  int64_t table_stride;
+  const int* kv_lens;   // [n]: cached tokens, the call's new ones included
+  const int* q_starts;  // [n + 1], or null: one new token per sequence
+  int n, max_pages, tokens;
+};
+
+// The first new token of sequence s (q_starts as given may hold anything: the
+// kernels only ever use values brought into [0, tokens]).
+__device__ __forceinline__ int seq_start(const SeqView& v, int s) {
+  if (!v.q_starts) return s < v.tokens ? s : v.tokens;
+  const int a = v.q_starts[s];
+  return a < 0 ? 0 : a > v.tokens ? v.tokens : a;
+}
+
+// The page of token `tok` of the sequence with page row `row`, or -1 where
+// there is none (past the table, or an entry outside the cache).
+__device__ __forceinline__ int page_of(const int* row, int max_pages, const CacheView& c, int tok) {
+  const int at = fdiv(tok, c.page_div);
+  if (at >= max_pages) return -1;
+  const int p = row[at];
+  return (unsigned)p < (uint64_t)c.n_pages ? p : -1;
+}
+
+rtenhip_status cache_view(const rtenhip_kv_cache* cache, CacheView& v, int& dtype);
+rtenhip_status seq_view(const rtenhip_sequences* seqs, int64_t tokens, SeqView& v);
+// q / k / v / out rows [tokens, heads, dim]: f32, unit stride along dim, rows
+// on 16 bytes.
+rtenhip_status check_rows(const rtenhip_tensor* t, int64_t tokens, int64_t heads, int64_t dim, const char* shape_msg,
+                          const char* align_msg);
+// Whether two views of [tokens, heads, dim] rows share memory without being
+// the same view.
+bool rows_clash(const rtenhip_tensor* a, const rtenhip_tensor* b);
+
+// Whether rows of `dim` elements at these strides, the extents n, are all apart
+// (what is written must not be written twice).
+bool rows_apart(const int64_t* n, const int64_t* strides, int count, int64_t dim);
+
+// Makes the context's device current for a launch and puts back the caller's.
+struct DeviceScope {
+  int before = -1;
+  rtenhip_status status = RTENHIP_OK;
+  explicit DeviceScope(int device) {
+    hipError_t e = hipGetDevice(&before);
+    if (e == hipSuccess && before == device) before = -1;
+    else if (e == hipSuccess) e = hipSetDevice(device);
+    if (e != hipSuccess) status = hip_fail(e, "hipSetDevice");
+  }
+  ~DeviceScope() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+}  // namespace rtenhip

@@ -1,0 +1,1223 @@
+// Attention of new tokens over a paged cache (rtenhip_paged_attention_f32).
+//
+//   out = sum_j softmax_j(scale q . k_j) v_j   over the tokens j that q sees,
+//
+// one pass over the keys and values with a running maximum m and sum l of the
+// softmax (base 2: q is multiplied by scale * log2 e once).  The query heads
+// that share a cache head are rows of one tile, so keys and values are read
+// once for all of them.
+//
+// A sequence with at most 16 rows (new tokens x heads of a group) runs in
+// decode_kernel, where the cache streams from memory straight into the
+// registers of the matrix instructions; the others run in chunk_kernel, 128
+// rows a workgroup, where a tile of 64 keys and values is shared through LDS.
+// Lengths live on the device, so each workgroup finds its own piece of work
+// (plan): the visible keys of all sequences, counted in tiles of 64, are
+// divided into stretches of about equal length, one to a workgroup.  Where a
+// tile of rows has several stretches, merge_kernel joins their results.
+#include "decoder.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace rtenhip {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int PA_THREADS = 256;
+constexpr int PA_UNIT = 64;    // keys of a tile
+constexpr int PA_SMALL = 16;   // rows of a decode tile
+constexpr int PA_BIG = 128;    // rows of a chunk tile
+constexpr float NEG_INF = -__builtin_huge_valf();
+
+// What merge_kernel has to know of a stretch.
+struct Part {
+  int slot, part, parts, stride;  // stretches of a tile are `stride` slots apart
+  int token0, row0, rows, head;
+};
+
+struct PagedDesc {
+  const float* q;
+  int64_t q_t, q_h;
+  float* out;
+  int64_t o_t, o_h;
+  CacheView c;
+  SeqView s;
+  FastDiv group_div;
+  int group, window, sinks;
+  float scale_log2e;
+  float minus1;  // -1, where the compiler must not know it (see split16)
+  int small_only;  // every sequence has at most PA_SMALL rows
+  // Workspace: the stretches of the decode grid, then those of the chunk grid.
+  int grid_small, grid_big, slots_small, slots_big;
+  int target_small, target_big;
+  Part* part_small;
+  Part* part_big;
+  float* o_small;  // [slots][PA_SMALL][dim] normalised results
+  float* o_big;    // [slots][PA_BIG][dim]
+  float2* ml_small;  // [slots][PA_SMALL] (m, l)
+  float2* ml_big;
+};
+
+// ---- plan ------------------------------------------------------------------------
+
+// The tiles of 64 keys that positions p0 .. p1 see: `sinks` whole tiles from 0
+// and then those from lo on.
+struct Span {
+  int sink_tiles, lo_tile, tiles;
+  int lo, end;  // keys in [0, sinks) and [lo, end) are seen by some row
+  __device__ __forceinline__ int tile(int i) const { return i < sink_tiles ? i : i - sink_tiles + lo_tile; }
+};
+
+__device__ __forceinline__ Span span_of(const PagedDesc& d, int kv_len, int p0, int p1) {
+  Span v;
+  // (A tile's last key stays below 2^31.)
+  const int64_t room = min((int64_t)d.s.max_pages * d.c.page_size, (int64_t)0x7fffff00);
+  int end = kv_len < room ? kv_len : (int)room;
+  end = min(end, p1 + 1);
+  v.end = max(end, 0);
+  v.lo = 0;
+  v.sink_tiles = 0;
+  if (d.window) {
+    const int64_t lo = (int64_t)p0 - d.window + 1;
+    v.lo = lo < 0 ? 0 : (int)lo;
+    v.lo_tile = v.lo / PA_UNIT;
+    v.sink_tiles = min((min(d.sinks, v.end) + PA_UNIT - 1) / PA_UNIT, v.lo_tile);
+  }
+  v.lo_tile = v.lo / PA_UNIT;
+  v.tiles = v.sink_tiles + max(0, (v.end + PA_UNIT - 1) / PA_UNIT - v.lo_tile);
+  return v;
+}
+
+struct Work {
+  int seq, start, q_len, kv_len;
+  int tile, head, part, parts, slot;
+};
+
+struct SeqWork {
+  int start, q_len, kv_len, tiles, units;  // tiles of rows, tiles of keys
+};
+
+template <bool BIG>
+__device__ __forceinline__ SeqWork seq_work(const PagedDesc& d, int s) {
+  SeqWork w;
+  w.start = seq_start(d.s, s);
+  w.q_len = max(0, seq_start(d.s, s + 1) - w.start);
+  w.kv_len = max(0, d.s.kv_lens[s]);
+  const int64_t rows = (int64_t)w.q_len * d.group;
+  w.units = 0;
+  if (BIG)
+    w.tiles = rows > PA_SMALL ? (int)((rows + PA_BIG - 1) / PA_BIG) : 0;
+  else
+    w.tiles = rows > 0 && rows <= PA_SMALL;
+  if (w.tiles) w.units = max(1, span_of(d, w.kv_len, w.kv_len - w.q_len, w.kv_len - 1).tiles);
+  return w;
+}
+
+struct PlanShared {
+  int64_t units[4];
+  int items[4], slots[4];
+  Work work;
+};
+
+__device__ __forceinline__ int wave_scan(int x) {  // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const int y = __shfl_up(x, m);
+    if (lane >= m) x += y;
+  }
+  return x;
+}
+
+// The piece of work of workgroup `block`: false if there is none.  Every
+// workgroup counts for itself (thread i the sequences i * each ..), which
+// costs no launch and no order between workgroups.
+template <bool BIG>
+__device__ bool plan(const PagedDesc& d, int block, PlanShared& sh, Work& out) {
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int each = (d.s.n + PA_THREADS - 1) / PA_THREADS;
+  const int s0 = tid * each, s1 = min(d.s.n, s0 + each);
+  const int heads = d.c.heads;
+  int64_t units = 0;
+  for (int s = s0; s < s1; s++) {
+    const SeqWork w = seq_work<BIG>(d, s);
+    units += (int64_t)w.tiles * w.units;
+  }
+#pragma unroll
+  for (int m = 32; m; m >>= 1) units += __shfl_xor((long long)units, m);
+  if (lane == 0) sh.units[wave] = units;
+  if (tid == 0) sh.work.seq = -1;
+  __syncthreads();
+  const int64_t total = (sh.units[0] + sh.units[1] + sh.units[2] + sh.units[3]) * heads;
+  const int64_t target = BIG ? d.target_big : d.target_small;
+  // Keys of a stretch, in tiles: stretches for the whole card, none shorter
+  // than a tile.
+  const int64_t len64 = (total + target - 1) / target;
+  const int len = (int)(len64 < 1 ? 1 : len64 > (1 << 26) ? (1 << 26) : len64);
+  int items = 0, slots = 0;
+  for (int s = s0; s < s1; s++) {
+    const SeqWork w = seq_work<BIG>(d, s);
+    const int parts = (w.units + len - 1) / len;
+    const int n = w.tiles * heads * parts;
+    items += n;
+    slots += parts > 1 ? n : 0;
+  }
+  const int items_in = wave_scan(items), slots_in = wave_scan(slots);
+  if (lane == 63) sh.items[wave] = items_in, sh.slots[wave] = slots_in;
+  __syncthreads();
+  int at = items_in - items, slot = slots_in - slots;
+  for (int w = 0; w < wave; w++) at += sh.items[w], slot += sh.slots[w];
+  if (block >= at && block < at + items) {
+    for (int s = s0; s < s1; s++) {
+      const SeqWork w = seq_work<BIG>(d, s);
+      const int parts = (w.units + len - 1) / len;
+      const int n = w.tiles * heads * parts;
+      if (block < at + n) {
+        int i = block - at;
+        Work r;
+        r.seq = s, r.start = w.start, r.q_len = w.q_len, r.kv_len = w.kv_len;
+        r.slot = parts > 1 ? slot + i : -1;
+        r.head = i % heads;
+        i /= heads;
+        r.part = i % parts;
+        r.parts = parts;
+        r.tile = w.tiles - 1 - i / parts;  // the last rows see the most keys: first
+        sh.work = r;
+        break;
+      }
+      at += n;
+      slot += parts > 1 ? n : 0;
+    }
+  }
+  __syncthreads();
+  out = sh.work;
+  return out.seq >= 0;
+}
+
+// ---- small pieces ------------------------------------------------------------------
+
+__device__ __forceinline__ float half_max(float x) {  // with lane ^ 32
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float quarter_max(float x) {  // over lanes ^ 16, ^ 32
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quarter_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float wave_max(float x) {
+  x = fmaxf(x, dpp<0xB1>(x));   // lane ^ 1
+  x = fmaxf(x, dpp<0x4E>(x));   // lane ^ 2
+  x = fmaxf(x, dpp<0x141>(x));  // mirrored in its 8
+  x = fmaxf(x, dpp<0x140>(x));  // mirrored in its 16
+  return quarter_max(x);
+}
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// The power of two that brings a largest magnitude `big` to [2^13, 2^14), as
+// an exponent; what is not finite or very small counts as the nearest that is
+// in range, zero as 1.
+__device__ __forceinline__ int exponent_for(float big) {
+  int e = (int)((__float_as_uint(big) >> 23) & 255) - 127;
+  e = e > 127 ? 127 : e < -100 ? -100 : e;
+  return 13 - e;
+}
+__device__ __forceinline__ float pow2(int e) {  // e brought into the normal range
+  e = e < -126 ? -126 : e > 127 ? 127 : e;
+  return __uint_as_float((uint32_t)(e + 127) << 23);
+}
+
+// x = hi + lo in f16: 22 bits of x where |x| is within 2^14 and above 2^-3,
+// an absolute error of 2^-25 below that.  lo is x - hi exactly (one mixed
+// fma, hi times the -1 that is a register, before its own rounding).
+__device__ __forceinline__ void split16(float a, float b, float minus1, f16x2& hi, f16x2& lo) {
+  hi = (f16x2){(_Float16)a, (_Float16)b};
+  lo = (f16x2){(_Float16)__builtin_fmaf((float)hi[0], minus1, a), (_Float16)__builtin_fmaf((float)hi[1], minus1, b)};
+}
+
+template <int TYPE>
+struct CacheType {
+  static constexpr int size = TYPE == RTENHIP_CACHE_F32 ? 4 : 2;
+};
+
+// ---- decode --------------------------------------------------------------------------
+
+// Sixteen rows at most; each of the 4 waves takes 16 keys of every tile of 64
+// and keeps its own m, l and result, joined through LDS at the end.
+//  - S^T = K Q^T: lane (i, g) (i < 16, g < 4) loads parts of key i's row as
+//    they lie and feeds them to the matrix instruction as they are: which of
+//    the dimensions a step multiplies does not matter as long as Q's register
+//    holds the same ones.  The lane then has the scores of row i for the keys
+//    4g .. 4g + 3.
+//  - O^T = V^T P^T: those four are the P operand as they are, and the lane
+//    loads the values of keys 4g .. 4g + 3 for DP / 16 neighbouring
+//    dimensions, so nothing moves between lanes.
+// An f32 cache uses the f32 instructions, f16 splits q and p into two f16
+// terms (exact products, 22 bits of q and p), bf16 into three bf16 terms.
+// Bound by the cache's bytes: while one tile is worked on, the next tile's
+// keys and this one's values are on their way.
+template <int DP, int TYPE>
+struct DecodeTile {
+  static constexpr int DPL = DP / 16;                                // value dimensions of a lane
+  static constexpr int KV = DP * CacheType<TYPE>::size / 64;         // 16-byte loads of keys
+  static constexpr int VW = DPL * CacheType<TYPE>::size / 4;         // 32-bit words of values, per key
+  static constexpr int QW = TYPE == RTENHIP_CACHE_F32 ? DP / 4 : TYPE == RTENHIP_CACHE_F16 ? DP / 4 : 3 * DP / 8;
+};
+
+template <int DP, int TYPE>
+__device__ __forceinline__ void load_keys(const char* row, bool ok, int g, int dim, u32x4* k) {
+  constexpr int KV = DecodeTile<DP, TYPE>::KV, size = CacheType<TYPE>::size, per = 16 / size;
+#pragma unroll
+  for (int j = 0; j < KV; j++) {
+    const int at = (4 * j + g) * per;
+    k[j] = (u32x4){0, 0, 0, 0};
+    if (ok && at < dim) k[j] = *(const u32x4*)(row + at * size);
+  }
+}
+
+template <int DP, int TYPE>
+__device__ __forceinline__ void load_values(const char* row, bool ok, int i, int dim, uint32_t* v) {
+  constexpr int VW = DecodeTile<DP, TYPE>::VW, DPL = DP / 16, size = CacheType<TYPE>::size;
+  if constexpr (VW == 2) {
+    u32x2 x = {0, 0};
+    if (ok && i * DPL < dim) x = *(const u32x2*)(row + i * DPL * size);
+    v[0] = x[0], v[1] = x[1];
+  } else {
+#pragma unroll
+    for (int c = 0; c < VW / 4; c++) {
+      u32x4 x = {0, 0, 0, 0};
+      if (ok && i * DPL + c * (16 / size) < dim) x = *(const u32x4*)(row + i * DPL * size + c * 16);
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[4 * c + e] = x[e];
+    }
+  }
+}
+
+// The words of a key's or value's row with what is not finite set to zero;
+// true if there was any.
+template <int TYPE>
+__device__ __forceinline__ bool clean(uint32_t& w) {
+  if constexpr (TYPE == RTENHIP_CACHE_F32) {
+    const bool bad = (w & 0x7f800000u) == 0x7f800000u;
+    if (bad) w = 0;
+    return bad;
+  } else {
+    constexpr uint32_t e = TYPE == RTENHIP_CACHE_F16 ? 0x7c00u : 0x7f80u;
+    const bool lo = (w & e) == e, hi = (w & (e << 16)) == (e << 16);
+    if (lo) w &= 0xffff0000u;
+    if (hi) w &= 0x0000ffffu;
+    return lo || hi;
+  }
+}
+
+template <int DP, int TYPE>
+__global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(PagedDesc d) {
+  using T = DecodeTile<DP, TYPE>;
+  constexpr int DPL = T::DPL, KV = T::KV, VW = T::VW, size = CacheType<TYPE>::size;
+  __shared__ PlanShared plan_sh;
+  __shared__ float o_sh[4][PA_SMALL][DP];
+  __shared__ float m_sh[4][PA_SMALL], l_sh[4][PA_SMALL];
+  Work w;
+  const bool any = plan<false>(d, blockIdx.x, plan_sh, w);
+  if (threadIdx.x == 0 && d.part_small) {
+    Part p{};
+    if (any && w.slot >= 0 && w.slot < d.slots_small)
+      p = Part{w.slot, w.part, w.parts, d.c.heads, w.start, 0, w.q_len * d.group, w.head};
+    d.part_small[blockIdx.x] = p;
+  }
+  if (!any || w.slot >= d.slots_small) return;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int i = lane & 15, g = lane >> 4;
+  const int dim = d.c.dim, rows = w.q_len * d.group;
+  const int token = fdiv(i, d.group_div), sub = i - token * d.group;
+  const bool row_ok = i < rows;
+  const int pos = row_ok ? w.kv_len - w.q_len + token : -1;
+  const int64_t below = d.window ? (int64_t)pos - d.window : -1;  // keys up to here are seen as sinks only
+
+  // Q, times scale log2 e, as the matrix instructions take it.
+  uint32_t qw[T::QW];
+  float q_back = 1.f;  // what the scores are multiplied by
+  {
+    const float* q = d.q + (int64_t)(w.start + token) * d.q_t + (int64_t)(w.head * d.group + sub) * d.q_h;
+    constexpr int PER = 16 / size;
+    float x[KV][PER];
+#pragma unroll
+    for (int j = 0; j < KV; j++) {
+      const int at = (4 * j + g) * PER;
+      const bool ok = row_ok && at < dim;
+#pragma unroll
+      for (int e = 0; e < PER; e += 4) {
+        const float4 y = ok ? *(const float4*)(q + at + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[j][e] = y.x * d.scale_log2e, x[j][e + 1] = y.y * d.scale_log2e;
+        x[j][e + 2] = y.z * d.scale_log2e, x[j][e + 3] = y.w * d.scale_log2e;
+      }
+    }
+    if constexpr (TYPE == RTENHIP_CACHE_F32) {
+#pragma unroll
+      for (int j = 0; j < KV; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) qw[4 * j + e] = __float_as_uint(x[j][e]);
+    } else if constexpr (TYPE == RTENHIP_CACHE_F16) {
+      float big = 0.f;
+#pragma unroll
+      for (int j = 0; j < KV; j++)
+#pragma unroll
+        for (int e = 0; e < PER; e++) big = fmaxf(big, fabsf(x[j][e]));
+      const int up = exponent_for(quarter_max(big));
+      const float f = pow2(up);
+      q_back = pow2(-up);
+#pragma unroll
+      for (int j = 0; j < KV; j++)
+#pragma unroll
+        for (int e = 0; e < PER; e += 2) {
+          f16x2 hi, lo;
+          split16(x[j][e] * f, x[j][e + 1] * f, d.minus1, hi, lo);
+          qw[4 * j + e / 2] = __builtin_bit_cast(uint32_t, hi);
+          qw[DP / 8 + 4 * j + e / 2] = __builtin_bit_cast(uint32_t, lo);
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < KV; j++)
+#pragma unroll
+        for (int e = 0; e < PER; e += 2) {
+          float a = x[j][e], b = x[j][e + 1];
+#pragma unroll
+          for (int t = 0; t < 3; t++) {
+            const __bf16 ha = (__bf16)a, hb = (__bf16)b;
+            qw[t * DP / 8 + 4 * j + e / 2] = (uint32_t)__builtin_bit_cast(uint16_t, ha) |
+                                             (uint32_t)__builtin_bit_cast(uint16_t, hb) << 16;
+            a -= (float)ha, b -= (float)hb;
+          }
+        }
+    }
+  }
+
+  const Span span = span_of(d, w.kv_len, w.kv_len - w.q_len, w.kv_len - 1);
+  const int u0 = (int)((int64_t)span.tiles * w.part / w.parts), u1 = (int)((int64_t)span.tiles * (w.part + 1) / w.parts);
+  const int* table = d.s.table + (int64_t)w.seq * d.s.table_stride;
+  const char* kc = d.c.k + (int64_t)w.head * d.c.k_head * size;
+  const char* vc = d.c.v + (int64_t)w.head * d.c.v_head * size;
+
+  // The page of the lane's key (key i of the wave's 16) in tile u, -1 where no
+  // row sees the key.
+  auto page_at = [&](int u, int& key) {
+    key = 0;
+    if (u >= u1) return -1;
+    key = span.tile(u) * PA_UNIT + 16 * wave + i;
+    if (key >= span.end || (key < span.lo && key >= d.sinks)) return -1;
+    return page_of(table, d.s.max_pages, d.c, key);
+  };
+  auto slot_of = [&](int key) { return key - fdiv(key, d.c.page_div) * d.c.page_size; };
+
+  float m, l;
+  f32x4 o[DPL];
+  bool poison;
+  auto pass = [&](bool careful) {
+    m = NEG_INF, l = 0.f;
+    poison = false;
+#pragma unroll
+    for (int e = 0; e < DPL; e++) o[e] = (f32x4){0, 0, 0, 0};
+    int key, key_next;
+    int page = page_at(u0, key), page_next = page_at(u0 + 1, key_next);
+    u32x4 k[KV], k_next[KV];
+    load_keys<DP, TYPE>(kc + ((int64_t)page * d.c.k_page + (int64_t)slot_of(key) * d.c.k_slot) * size, page >= 0, g,
+                        dim, k);
+    for (int u = u0; u < u1; u++) {
+      // This tile's values, the next one's keys, the one after's pages.
+      int vpage[4];
+      uint32_t v[4][VW];
+      const int base = span.tile(u) * PA_UNIT + 16 * wave + 4 * g;
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        vpage[r] = __shfl(page, 4 * g + r);
+        load_values<DP, TYPE>(vc + ((int64_t)vpage[r] * d.c.v_page + (int64_t)slot_of(base + r) * d.c.v_slot) * size,
+                              vpage[r] >= 0, i, dim, v[r]);
+      }
+      load_keys<DP, TYPE>(
+          kc + ((int64_t)page_next * d.c.k_page + (int64_t)slot_of(key_next) * d.c.k_slot) * size, page_next >= 0, g,
+          dim, k_next);
+      page = page_next;
+      page_next = page_at(u + 2, key_next);
+
+      f32x4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < KV; j++) {
+        if constexpr (TYPE == RTENHIP_CACHE_F32) {
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            s0 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[j][e]), __uint_as_float(qw[4 * j + e]), s0, 0,
+                                                      0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[j][e + 1]), __uint_as_float(qw[4 * j + e + 1]),
+                                                      s1, 0, 0, 0);
+          }
+        } else {
+          const u32x4 a = k[j];
+          const auto part = [&](int t) {
+            return (u32x4){qw[t * DP / 8 + 4 * j], qw[t * DP / 8 + 4 * j + 1], qw[t * DP / 8 + 4 * j + 2],
+                           qw[t * DP / 8 + 4 * j + 3]};
+          };
+          if constexpr (TYPE == RTENHIP_CACHE_F16) {
+            const f16x8 x = __builtin_bit_cast(f16x8, a);
+            s0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, __builtin_bit_cast(f16x8, part(0)), s0, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, __builtin_bit_cast(f16x8, part(1)), s1, 0, 0, 0);
+          } else {
+            const bf16x8 x = __builtin_bit_cast(bf16x8, a);
+            s0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, part(0)), s0, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, part(1)), s1, 0, 0, 0);
+            s1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, part(2)), s1, 0, 0, 0);
+          }
+        }
+      }
+      float p[4], top = NEG_INF;
+      bool seen[4];
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int at = base + r;
+        seen[r] = vpage[r] >= 0 && at <= pos && (at > below || at < d.sinks);
+        p[r] = seen[r] ? (s0[r] + s1[r]) * q_back : NEG_INF;
+        top = fmaxf(top, p[r]);
+      }
+      const float m_new = fmaxf(m, quarter_max(top));
+      const float ref = m_new == NEG_INF ? 0.f : m_new;
+      const float fade = __builtin_amdgcn_exp2f(m - ref);
+      m = m_new;
+      // f16 terms of p have the most bits where the largest p is 2^14; the
+      // factor is in l too.
+      constexpr float UP = TYPE == RTENHIP_CACHE_F16 ? 14.f : 0.f;
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        p[r] = __builtin_amdgcn_exp2f((p[r] - ref) + UP);
+        sum += p[r];
+      }
+      l = __fmaf_rn(l, fade, sum);
+#pragma unroll
+      for (int e = 0; e < DPL; e++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) o[e][r] *= fade;
+      if (careful) {
+        // A value that is not finite must not meet the zero weight of a row
+        // that does not see it; the rows that do see it end as NaN.
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          bool bad = false;
+#pragma unroll
+          for (int c = 0; c < VW; c++) bad |= clean<TYPE>(v[r][c]);
+          const bool key_bad = (__ballot(bad) >> (16 * g)) & 0xffff;
+          poison |= key_bad && seen[r];
+        }
+      }
+      if constexpr (TYPE == RTENHIP_CACHE_F32) {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int e = 0; e < DPL; e++)
+            o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[r][e]), p[r], o[e], 0, 0, 0);
+      } else {
+        // Four keys' values of a dimension side by side.
+        const auto column = [&](int e) {
+          const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+          return (u32x2){__builtin_amdgcn_perm(v[1][e / 2], v[0][e / 2], sel),
+                         __builtin_amdgcn_perm(v[3][e / 2], v[2][e / 2], sel)};
+        };
+        if constexpr (TYPE == RTENHIP_CACHE_F16) {
+          f16x2 h0, l0, h1, l1;
+          split16(p[0], p[1], d.minus1, h0, l0);
+          split16(p[2], p[3], d.minus1, h1, l1);
+          const f16x4 hi = {h0[0], h0[1], h1[0], h1[1]}, lo = {l0[0], l0[1], l1[0], l1[1]};
+#pragma unroll
+          for (int e = 0; e < DPL; e++) {
+            const f16x4 a = __builtin_bit_cast(f16x4, column(e));
+            o[e] = __builtin_amdgcn_mfma_f32_16x16x16f16(a, hi, o[e], 0, 0, 0);
+            o[e] = __builtin_amdgcn_mfma_f32_16x16x16f16(a, lo, o[e], 0, 0, 0);
+          }
+        } else {
+          s16x4 terms[3];
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            float x = p[r];
+#pragma unroll
+            for (int t = 0; t < 3; t++) {
+              const __bf16 h = (__bf16)x;
+              terms[t][r] = __builtin_bit_cast(short, h);
+              x -= (float)h;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < DPL; e++) {
+            const s16x4 a = __builtin_bit_cast(s16x4, column(e));
+#pragma unroll
+            for (int t = 0; t < 3; t++) o[e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, terms[t], o[e], 0, 0, 0);
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < KV; j++) k[j] = k_next[j];
+    }
+    l = quarter_sum(l);
+  };
+  // A result that is not finite may come from a value that its row does not
+  // see: once more, with care.
+  for (int k = 0; k < 2; k++) {
+    pass(k);
+    bool bad = !finite(l);
+#pragma unroll
+    for (int e = 0; e < DPL; e++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) bad |= !finite(o[e][r]);
+    if (!__any(bad)) break;
+  }
+  if (quarter_max(poison ? 1.f : 0.f) > 0.f) l = __builtin_nanf("");
+  if (g == 0) m_sh[wave][i] = m, l_sh[wave][i] = l;
+#pragma unroll
+  for (int r = 0; r < 4; r++)
+#pragma unroll
+    for (int e = 0; e < DPL; e += 4)
+      *(f32x4*)&o_sh[wave][i][DPL * (4 * g + r) + e] = (f32x4){o[e][r], o[e + 1][r], o[e + 2][r], o[e + 3][r]};
+  __syncthreads();
+  const int quads = dim / 4;
+  for (int at = tid; at < rows * quads; at += PA_THREADS) {
+    const int row = at / quads, c = (at - row * quads) * 4;
+    const float m_all = fmaxf(fmaxf(m_sh[0][row], m_sh[1][row]), fmaxf(m_sh[2][row], m_sh[3][row]));
+    const float ref = m_all == NEG_INF ? 0.f : m_all;
+    f32x4 sum = {0, 0, 0, 0};
+    float l_all = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const float f = __builtin_amdgcn_exp2f(m_sh[k][row] - ref);
+      l_all = __fmaf_rn(l_sh[k][row], f, l_all);
+      const f32x4 x = *(const f32x4*)&o_sh[k][row][c];
+#pragma unroll
+      for (int e = 0; e < 4; e++) sum[e] = __fmaf_rn(x[e], f, sum[e]);
+    }
+    const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+#pragma unroll
+    for (int e = 0; e < 4; e++) sum[e] *= inv;
+    if (w.slot < 0) {
+      const int tok = row / d.group;
+      *(f32x4*)(d.out + (int64_t)(w.start + tok) * d.o_t + (int64_t)(w.head * d.group + row - tok * d.group) * d.o_h +
+                c) = sum;
+    } else {
+      *(f32x4*)(d.o_small + ((int64_t)w.slot * PA_SMALL + row) * dim + c) = sum;
+      if (c == 0) d.ml_small[(int64_t)w.slot * PA_SMALL + row] = make_float2(m_all, l_all);
+    }
+  }
+}
+
+// ---- chunk ---------------------------------------------------------------------------
+
+// 128 rows (new token, head of the group) a workgroup, 32 a wave.  A tile of
+// 64 keys and values goes to LDS as f16 terms, and both products run on the
+// f16 matrix instructions:
+//  - an f32 number x 2^e is hi + lo, each f16 (split16), and a product
+//    hi hi + hi lo + lo hi, three f16 instructions against the eight times
+//    longer f32 one, loses what is below 2^-22 of it; a 16-bit cache needs no
+//    lo.  e is one power of two for the tile's keys and one, which only ever
+//    grows, for the values so far, so the largest number of either is near
+//    2^13 and the terms are exact to 2^-38 of it; q has one for each row, p
+//    the factor 2^8.  Powers of two come out again exactly.
+//  - S^T = K Q^T: a lane (n, h) has row n's scores for the keys
+//    8 i + 4 h + j of each 32, so the softmax needs one exchange with lane
+//    ^ 32, and
+//  - O^T = V^T P^T takes them as they lie: LDS holds V^T with the keys of
+//    every 16 in the order (h, i, j), 16 bytes for a lane's eight.
+//  The maximum that p is taken against follows the largest score only when it
+//  is passed by more than 2^6, which few tiles do, so the result is hardly
+//  ever rescaled.
+// Bound by the matrix instructions at long prompts; two workgroups on a CU,
+// so that one's loads, maxima and conversions run under the other's products.
+template <int DP, int TYPE>
+struct ChunkTile {
+  static constexpr int TERMS = TYPE == RTENHIP_CACHE_F32 ? 2 : 1;
+  static constexpr int KS = DP * 2 + 16;  // bytes of a key's row in LDS, off by a bank group per row
+  static constexpr int KL = DP * CacheType<TYPE>::size / 64;          // 16-byte loads of keys per thread
+  static constexpr int VW = DP / 16 * CacheType<TYPE>::size / 4;      // words of values per thread and key
+  static constexpr int K_BYTES = PA_UNIT * KS, V_BYTES = DP * PA_UNIT * 2;
+};
+
+// Where the 16 bytes of keys (h, i, j), chunk = 2 * (16 keys) + h, of a
+// dimension lie: the chunks of neighbouring dimensions, and of dimensions 8
+// apart, are in different banks.
+__device__ __forceinline__ int value_at(int dimension, int chunk) {
+  return dimension * (PA_UNIT * 2) + ((chunk ^ dimension ^ (dimension >> 3)) & 7) * 16;
+}
+
+template <int TYPE>
+__device__ __forceinline__ float cache_lo(uint32_t w) {
+  if constexpr (TYPE == RTENHIP_CACHE_F16) return (float)__builtin_bit_cast(f16x2, w)[0];
+  return __uint_as_float(w << 16);
+}
+template <int TYPE>
+__device__ __forceinline__ float cache_hi(uint32_t w) {
+  if constexpr (TYPE == RTENHIP_CACHE_F16) return (float)__builtin_bit_cast(f16x2, w)[1];
+  return __uint_as_float(w & 0xffff0000u);
+}
+
+// The largest magnitude in a word of the cache and `top`.
+template <int TYPE>
+__device__ __forceinline__ float top_of(float top, uint32_t w) {
+  if constexpr (TYPE == RTENHIP_CACHE_F32) return fmaxf(top, fabsf(__uint_as_float(w)));
+  return fmaxf(top, fmaxf(fabsf(cache_lo<TYPE>(w)), fabsf(cache_hi<TYPE>(w))));
+}
+
+template <int DP, int TYPE>
+__global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void chunk_kernel(PagedDesc d) {
+  using T = ChunkTile<DP, TYPE>;
+  constexpr int TERMS = T::TERMS, KS = T::KS, KL = T::KL, VW = T::VW, DPL = DP / 16;
+  constexpr int size = CacheType<TYPE>::size, PER = 16 / size, NB = DP / 32;
+  constexpr bool SCALED = TYPE != RTENHIP_CACHE_F16;  // f16 rows go to LDS as they are
+  __shared__ PlanShared plan_sh;
+  __shared__ __attribute__((aligned(16))) char k_sh[TERMS][T::K_BYTES];
+  __shared__ __attribute__((aligned(16))) char v_sh[TERMS][T::V_BYTES];
+  __shared__ float top_sh[2][4];
+  __shared__ int hole_sh[4];
+  __shared__ __attribute__((aligned(4))) uint8_t seen_sh[PA_UNIT], bad_sh[PA_UNIT];
+  Work w;
+  const bool any = plan<true>(d, blockIdx.x, plan_sh, w);
+  const int row0 = w.tile * PA_BIG;
+  const int all_rows = any ? w.q_len * d.group : 0;
+  const int rows = min(PA_BIG, all_rows - row0);
+  if (threadIdx.x == 0 && d.part_big) {
+    Part p{};
+    if (any && w.slot >= 0 && w.slot < d.slots_big)
+      p = Part{w.slot, w.part, w.parts, d.c.heads, w.start, row0, rows, w.head};
+    d.part_big[blockIdx.x] = p;
+  }
+  if (!any || w.slot >= d.slots_big) return;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int n = lane & 31, h = lane >> 5;
+  const int dim = d.c.dim, first = w.kv_len - w.q_len;
+  const int wave_row = row0 + wave * 32;
+  const bool wave_ok = wave_row < all_rows;
+  const int row = wave_row + n;
+  const bool row_ok = row < all_rows;
+  const int token = fdiv(row_ok ? row : 0, d.group_div), sub = row_ok ? row - token * d.group : 0;
+  const int pos = row_ok ? first + token : -1;
+  const int64_t below = d.window ? (int64_t)pos - d.window : -1;
+  // The first and the last position of the wave's rows.
+  const int pos_lo = wave_ok ? first + fdiv(wave_row, d.group_div) : 0;
+  const int pos_hi = wave_ok ? first + fdiv(min(wave_row + 31, all_rows - 1), d.group_div) : -1;
+
+  f16x8 q_hi[DP / 16], q_lo[DP / 16];
+  int q_up;
+  {
+    const float* q = d.q + (int64_t)(w.start + token) * d.q_t + (int64_t)(w.head * d.group + sub) * d.q_h;
+    float x[DP / 16][8], top = 0.f;
+#pragma unroll
+    for (int j = 0; j < DP / 16; j++) {
+      const int at = 16 * j + 8 * h;
+      const bool ok = row_ok && at < dim;
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const float4 y = ok ? *(const float4*)(q + at + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[j][e] = y.x * d.scale_log2e, x[j][e + 1] = y.y * d.scale_log2e;
+        x[j][e + 2] = y.z * d.scale_log2e, x[j][e + 3] = y.w * d.scale_log2e;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[j][e]));
+    }
+    q_up = exponent_for(half_max(top));
+    const float f = pow2(q_up);
+#pragma unroll
+    for (int j = 0; j < DP / 16; j++)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        f16x2 hi, lo;
+        split16(x[j][e] * f, x[j][e + 1] * f, d.minus1, hi, lo);
+        q_hi[j][e] = hi[0], q_hi[j][e + 1] = hi[1];
+        q_lo[j][e] = lo[0], q_lo[j][e + 1] = lo[1];
+      }
+  }
+
+  const Span span = span_of(d, w.kv_len, first + fdiv(row0, d.group_div),
+                            first + fdiv(row0 + rows - 1, d.group_div));
+  const int u0 = (int)((int64_t)span.tiles * w.part / w.parts), u1 = (int)((int64_t)span.tiles * (w.part + 1) / w.parts);
+  const int* table = d.s.table + (int64_t)w.seq * d.s.table_stride;
+  const char* kc = d.c.k + (int64_t)w.head * d.c.k_head * size;
+  const char* vc = d.c.v + (int64_t)w.head * d.c.v_head * size;
+
+  // Staging: keys, thread (row, quarter); values, thread (4 keys, DP / 16
+  // dimensions).
+  const int k_row = tid >> 2, k_quarter = tid & 3, v_four = tid >> 4, v_group = tid & 15;
+  auto seen_key = [&](int key) { return key < span.end && (key >= span.lo || key < d.sinks); };
+  auto page_at = [&](int u, int at) {
+    if (u >= u1) return -1;
+    const int key = span.tile(u) * PA_UNIT + at;
+    return seen_key(key) ? page_of(table, d.s.max_pages, d.c, key) : -1;
+  };
+  auto slot_of = [&](int key) { return key - fdiv(key, d.c.page_div) * d.c.page_size; };
+  u32x4 k_in[KL];
+  uint32_t v_in[4][VW];
+  int k_page, v_page[4];
+  auto find_pages = [&](int u) {
+    k_page = page_at(u, k_row);
+#pragma unroll
+    for (int r = 0; r < 4; r++) v_page[r] = page_at(u, 4 * v_four + r);
+  };
+  bool k_here, k_hole;  // the row in flight: a key somebody sees; one that would be seen but has no page
+  auto load = [&](int u) {
+    const int base = u < u1 ? span.tile(u) * PA_UNIT : 0;
+    k_here = k_page >= 0;
+    k_hole = u < u1 && !k_here && seen_key(base + k_row);
+    const char* kr = kc + ((int64_t)k_page * d.c.k_page + (int64_t)slot_of(base + k_row) * d.c.k_slot) * size;
+#pragma unroll
+    for (int j = 0; j < KL; j++) {
+      const int at = (4 * j + k_quarter) * PER;
+      k_in[j] = (u32x4){0, 0, 0, 0};
+      if (k_here && at < dim) k_in[j] = *(const u32x4*)(kr + at * size);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+      load_values<DP, TYPE>(
+          vc + ((int64_t)v_page[r] * d.c.v_page + (int64_t)slot_of(base + 4 * v_four + r) * d.c.v_slot) * size,
+          v_page[r] >= 0, v_group, dim, v_in[r]);
+  };
+
+  float m, l;
+  f32x16 o[NB];
+  int v_up;
+  bool poison;
+  auto pass = [&](bool careful) {
+    m = NEG_INF, l = 0.f;
+    v_up = 113;  // as for values that are all zero or very small
+    poison = false;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) o[b][e] = 0.f;
+    find_pages(u0);
+    load(u0);
+    find_pages(u0 + 1);
+    for (int u = u0; u < u1; u++) {
+      const int base = span.tile(u) * PA_UNIT;
+      bool v_bad[4] = {false, false, false, false};
+      if (careful) {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int c = 0; c < VW; c++) v_bad[r] |= clean<TYPE>(v_in[r][c]);
+      }
+      float k_top = 0.f, v_top = 0.f;
+      if constexpr (SCALED) {
+#pragma unroll
+        for (int j = 0; j < KL; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            uint32_t x = k_in[j][e];
+            if (careful) clean<TYPE>(x);
+            k_top = top_of<TYPE>(k_top, x);
+          }
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int c = 0; c < VW; c++) v_top = top_of<TYPE>(v_top, v_in[r][c]);
+        k_top = wave_max(k_top);
+        v_top = wave_max(v_top);
+        if (lane == 0) top_sh[0][wave] = k_top, top_sh[1][wave] = v_top;
+      }
+      const bool hole = __any(k_hole);
+      if (lane == 0) hole_sh[wave] = hole;
+      // Everybody is through with the tile before, and the tops are there.
+      __syncthreads();
+      int k_up = 0;
+      float v_f = 1.f;
+      if constexpr (SCALED) {
+        k_up = exponent_for(fmaxf(fmaxf(top_sh[0][0], top_sh[0][1]), fmaxf(top_sh[0][2], top_sh[0][3])));
+        const int up = exponent_for(fmaxf(fmaxf(top_sh[1][0], top_sh[1][1]), fmaxf(top_sh[1][2], top_sh[1][3])));
+        if (up < v_up) {  // larger values than any before: one binade of room more
+          const float f = pow2(up - 1 - v_up);
+          v_up = up - 1;
+#pragma unroll
+          for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[b][e] *= f;
+        }
+        v_f = pow2(v_up);
+      }
+      const bool holes = hole_sh[0] | hole_sh[1] | hole_sh[2] | hole_sh[3];
+      {
+        const float k_f = pow2(k_up);
+        char* to = &k_sh[0][k_row * KS];
+#pragma unroll
+        for (int j = 0; j < KL; j++) {
+          const int at = (4 * j + k_quarter) * PER * 2;
+          if constexpr (TYPE == RTENHIP_CACHE_F16) {
+            *(u32x4*)(to + at) = k_in[j];
+          } else if constexpr (TYPE == RTENHIP_CACHE_BF16) {
+            u32x4 y;
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              y[e] = __builtin_bit_cast(uint32_t, (f16x2){(_Float16)(cache_lo<TYPE>(k_in[j][e]) * k_f),
+                                                          (_Float16)(cache_hi<TYPE>(k_in[j][e]) * k_f)});
+            *(u32x4*)(to + at) = y;
+          } else {
+            f16x2 h0, l0, h1, l1;
+            split16(__uint_as_float(k_in[j][0]) * k_f, __uint_as_float(k_in[j][1]) * k_f, d.minus1, h0, l0);
+            split16(__uint_as_float(k_in[j][2]) * k_f, __uint_as_float(k_in[j][3]) * k_f, d.minus1, h1, l1);
+            *(f16x4*)(to + at) = (f16x4){h0[0], h0[1], h1[0], h1[1]};
+            *(f16x4*)(to + T::K_BYTES + at) = (f16x4){l0[0], l0[1], l1[0], l1[1]};
+          }
+        }
+        // Keys 4 v_four ..: the 16 they are in, h and i (value_at).
+        const int chunk = (v_four >> 2) * 2 + (v_four & 1), half = (v_four >> 1 & 1) * 8;
+        char* vt = &v_sh[0][half];
+#pragma unroll
+        for (int e = 0; e < DPL; e++) {
+          const int at = value_at(DPL * v_group + e, chunk);
+          if constexpr (TYPE == RTENHIP_CACHE_F16) {
+            const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+            *(u32x2*)(vt + at) = (u32x2){__builtin_amdgcn_perm(v_in[1][e / 2], v_in[0][e / 2], sel),
+                                         __builtin_amdgcn_perm(v_in[3][e / 2], v_in[2][e / 2], sel)};
+          } else if constexpr (TYPE == RTENHIP_CACHE_BF16) {
+            float x[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+              x[r] = (e & 1 ? cache_hi<TYPE>(v_in[r][e / 2]) : cache_lo<TYPE>(v_in[r][e / 2])) * v_f;
+            *(f16x4*)(vt + at) = (f16x4){(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+          } else {
+            f16x2 h0, l0, h1, l1;
+            split16(__uint_as_float(v_in[0][e]) * v_f, __uint_as_float(v_in[1][e]) * v_f, d.minus1, h0, l0);
+            split16(__uint_as_float(v_in[2][e]) * v_f, __uint_as_float(v_in[3][e]) * v_f, d.minus1, h1, l1);
+            *(f16x4*)(vt + at) = (f16x4){h0[0], h0[1], h1[0], h1[1]};
+            *(f16x4*)(vt + T::V_BYTES + at) = (f16x4){l0[0], l0[1], l1[0], l1[1]};
+          }
+        }
+        if (k_quarter == 0) seen_sh[k_row] = k_here;
+        if (careful) {
+          if (tid < PA_UNIT) bad_sh[tid] = 0;
+        }
+      }
+      __syncthreads();
+      if (careful) {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          if (v_bad[r]) bad_sh[4 * v_four + r] = 1;
+        __syncthreads();
+      }
+      load(u + 1);
+      find_pages(u + 2);
+
+      // Tiles past all of the wave's rows, or before all their windows.
+      const int64_t below_lo = d.window ? (int64_t)pos_lo - d.window : -1;
+      if (!wave_ok || base > pos_hi || (d.window && base + PA_UNIT - 1 <= below_lo && base >= d.sinks)) continue;
+      const int64_t below_hi = d.window ? (int64_t)pos_hi - d.window : -1;
+      const bool whole = !holes && !careful && wave_row + 31 < all_rows && base + PA_UNIT - 1 <= pos_lo &&
+                         base + PA_UNIT <= span.end &&
+                         (base > below_hi || base + PA_UNIT <= d.sinks);
+      const float back = pow2(-q_up - k_up);
+#pragma unroll
+      for (int tb = 0; tb < 2; tb++) {
+        f32x16 s;
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[e] = 0.f;
+        const char* kr = &k_sh[0][(32 * tb + n) * KS + 16 * h];
+#pragma unroll
+        for (int j = 0; j < DP / 16; j++) {
+          const f16x8 a = *(const f16x8*)(kr + 32 * j);
+          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q_hi[j], s, 0, 0, 0);
+          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q_lo[j], s, 0, 0, 0);
+          if constexpr (TERMS == 2) {
+            const f16x8 b = *(const f16x8*)(kr + T::K_BYTES + 32 * j);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, q_hi[j], s, 0, 0, 0);
+          }
+        }
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const int at = base + 32 * tb + 2 * e + 4 * h;
+            const uint32_t here = *(const uint32_t*)&seen_sh[32 * tb + 2 * e + 4 * h];
+            const uint32_t bad = careful ? *(const uint32_t*)&bad_sh[32 * tb + 2 * e + 4 * h] : 0;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              const bool seen = (here >> (8 * r) & 1) && at + r <= pos && (at + r > below || at + r < d.sinks);
+              if (!seen) s[e + r] = NEG_INF;
+              poison |= seen && (bad >> (8 * r) & 1);
+            }
+          }
+        }
+        float top = s[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) top = fmaxf(top, s[e]);
+        top = half_max(top) * back;
+        if (__any(top > m + 6.f)) {
+          const float m_new = fmaxf(m, top);
+          const float fade = __builtin_amdgcn_exp2f(m - (m_new == NEG_INF ? 0.f : m_new));
+          m = m_new;
+          l *= fade;
+#pragma unroll
+          for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[b][e] *= fade;
+        }
+        // p 2^8: at most 2^14.
+        const float ref = 8.f - (m == NEG_INF ? 0.f : m);
+        f16x8 p_hi[2], p_lo[2];
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const float a = __builtin_amdgcn_exp2f(__fmaf_rn(s[e], back, ref));
+          const float b = __builtin_amdgcn_exp2f(__fmaf_rn(s[e + 1], back, ref));
+          sum += a + b;
+          f16x2 hi, lo;
+          split16(a, b, d.minus1, hi, lo);
+          p_hi[e >> 3][e & 7] = hi[0], p_hi[e >> 3][(e & 7) + 1] = hi[1];
+          p_lo[e >> 3][e & 7] = lo[0], p_lo[e >> 3][(e & 7) + 1] = lo[1];
+        }
+        l += sum;
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+          for (int b = 0; b < NB; b++) {
+            const int at = value_at(32 * b + n, 2 * (2 * tb + c) + h);
+            const f16x8 a = *(const f16x8*)&v_sh[0][at];
+            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p_hi[c], o[b], 0, 0, 0);
+            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p_lo[c], o[b], 0, 0, 0);
+            if constexpr (TERMS == 2) {
+              const f16x8 z = *(const f16x8*)&v_sh[TERMS - 1][at];
+              o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(z, p_hi[c], o[b], 0, 0, 0);
+            }
+          }
+      }
+    }
+  };
+  for (int k = 0; k < 2; k++) {
+    pass(k);
+    bool bad = !finite(l);
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) bad |= !finite(o[b][e]);
+    if (!__syncthreads_or(bad && wave_ok)) break;
+  }
+  l = half_sum(l);
+  if (half_max(poison ? 1.f : 0.f) > 0.f) l = __builtin_nanf("");
+  if (!row_ok) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float v_back = SCALED ? pow2(-v_up) : 1.f;
+  const int r = wave * 32 + n;
+  float* to = w.slot < 0 ? d.out + (int64_t)(w.start + token) * d.o_t + (int64_t)(w.head * d.group + sub) * d.o_h
+                         : d.o_big + ((int64_t)w.slot * PA_BIG + r) * dim;
+  if (w.slot >= 0 && h == 0) d.ml_big[(int64_t)w.slot * PA_BIG + r] = make_float2(m, l);
+#pragma unroll
+  for (int b = 0; b < NB; b++)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      const int at = 32 * b + 2 * e + 4 * h;
+      if (at < dim)
+        *(f32x4*)(to + at) = (f32x4){o[b][e] * inv * v_back, o[b][e + 1] * inv * v_back, o[b][e + 2] * inv * v_back,
+                                     o[b][e + 3] * inv * v_back};
+    }
+}
+
+// ---- merge ---------------------------------------------------------------------------
+
+// out = sum_i l_i 2^(m_i - max m) o_i / sum_i l_i 2^(m_i - max m) over the
+// stretches of a tile.  Workgroup (slot, part) joins its share of the tile's
+// numbers, so a tile of many stretches is joined by as many workgroups.
+template <bool BIG>
+__global__ __launch_bounds__(PA_THREADS) void merge_kernel(PagedDesc d) {
+  constexpr int ROWS = BIG ? PA_BIG : PA_SMALL;
+  const Part p = (BIG ? d.part_big : d.part_small)[blockIdx.x];
+  if (p.parts < 2) return;
+  const float* os = BIG ? d.o_big : d.o_small;
+  const float2* ml = BIG ? d.ml_big : d.ml_small;
+  const int slot0 = p.slot - p.part * p.stride;
+  const int dim = d.c.dim, quads = dim / 4, n = p.rows * quads;
+  const int each = (n + p.parts - 1) / p.parts;
+  const int end = min(n, each * (p.part + 1));
+  for (int at = each * p.part + threadIdx.x; at < end; at += PA_THREADS) {
+    const int row = at / quads, c = (at - row * quads) * 4;
+    float m = NEG_INF, l = 0.f;
+    f32x4 sum = {0, 0, 0, 0};
+    for (int i = 0; i < p.parts; i++) {
+      const int64_t slot = slot0 + (int64_t)i * p.stride;
+      const float2 x = ml[slot * ROWS + row];
+      const f32x4 o = *(const f32x4*)(os + (slot * ROWS + row) * dim + c);
+      if (x.y == 0.f) continue;  // saw nothing
+      const float m_new = fmaxf(m, x.x);
+      const float a = __builtin_amdgcn_exp2f(m - m_new), b = __builtin_amdgcn_exp2f(x.x - m_new) * x.y;
+      m = m_new;
+      l = __fmaf_rn(l, a, b);
+#pragma unroll
+      for (int e = 0; e < 4; e++) sum[e] = __fmaf_rn(sum[e], a, b * o[e]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int r = p.row0 + row, token = fdiv(r, d.group_div), sub = r - token * d.group;
+#pragma unroll
+    for (int e = 0; e < 4; e++) sum[e] *= inv;
+    *(f32x4*)(d.out + (int64_t)(p.token0 + token) * d.o_t + (int64_t)(p.head * d.group + sub) * d.o_h + c) = sum;
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------
+
+constexpr int PA_TARGET_SMALL = 1024, PA_TARGET_BIG = 512;
+
+// Grids and workspace, from sizes the host knows.  tiles_s heads parts_s summed
+// over the sequences is at most target + the tiles, and a sequence with two
+// stretches or more has less than twice its share of the target.
+struct PagedPlan {
+  int64_t grid_small, grid_big, slots_small, slots_big;
+  size_t bytes;
+  int64_t part_small, part_big, ml_small, ml_big, o_small, o_big;  // offsets in bytes
+};
+
+static rtenhip_status paged_plan(const rtenhip_tensor* q, const rtenhip_kv_cache* cache, const rtenhip_sequences* seqs,
+                                 PagedDesc& d, int& dtype, PagedPlan& p) {
+  if (!q) return fail(RTENHIP_MISSING_INPUTS, "Missing input");
+  rtenhip_status st = cache_view(cache, d.c, dtype);
+  if (st) return st;
+  if (q->ndim != 3) return fail(RTENHIP_INCOMPATIBLE_INPUT_SHAPES, "Expected [tokens, heads, head_dim] inputs");
+  const int64_t tokens = q->shape[0], heads = q->shape[1];
+  if (tokens < 0 || heads < 1 || heads > 65536) return fail(RTENHIP_INVALID_VALUE, "Invalid input size");
+  if (heads % d.c.heads)
+    return fail(RTENHIP_INCOMPATIBLE_INPUT_SHAPES, "Query heads must be a multiple of the cache's");
+  const int64_t group = heads / d.c.heads;
+  // (Row numbers and grids stay below 2^31.)
+  if (tokens * heads > (int64_t(1) << 30)) return fail(RTENHIP_UNSUPPORTED_VALUE, "Too many query rows");
+  st = check_rows(q, tokens, heads, d.c.dim, "q must be [tokens, heads, head_dim] with the cache's head_dim",
+                  "Head rows must have unit stride and start on 16 bytes");
+  if (!st) st = seq_view(seqs, tokens, d.s);
+  if (st) return st;
+  d.group = (int)group;
+  d.group_div = make_fastdiv((uint32_t)group);
+  const int64_t n = seqs->n_seqs, hk = d.c.heads, dim = d.c.dim;
+  const int64_t longest = seqs->q_starts ? tokens : std::min<int64_t>(tokens, 1);  // new tokens of a sequence
+  const bool small = group <= PA_SMALL, big = longest * group > PA_SMALL;
+  // One stretch a tile where no sequence has more than one tile of keys.
+  const bool splits = (int64_t)seqs->max_pages * cache->page_size > PA_UNIT;
+  p = PagedPlan{};
+  if (tokens && n) {
+    const int64_t small_tiles = std::min(n, tokens) * hk;
+    const int64_t big_tiles = (tokens * group / PA_BIG + std::min(n, tokens)) * hk;
+    if (small) p.grid_small = small_tiles + (splits ? PA_TARGET_SMALL : 0);
+    if (big) p.grid_big = big_tiles + (splits ? PA_TARGET_BIG : 0);
+    if (p.grid_small > INT32_MAX || p.grid_big > INT32_MAX)
+      return fail(RTENHIP_UNSUPPORTED_VALUE, "Too many query rows");
+    if (splits) {
+      p.slots_small = small ? 2 * PA_TARGET_SMALL : 0;
+      p.slots_big = big ? 2 * PA_TARGET_BIG : 0;
+    }
+  }
+  size_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    const size_t here = at;
+    at += (size_t)((bytes + 255) / 256 * 256);
+    return (int64_t)here;
+  };
+  if (splits) {
+    p.part_small = take(p.grid_small * (int64_t)sizeof(Part));
+    p.part_big = take(p.grid_big * (int64_t)sizeof(Part));
+    p.ml_small = take(p.slots_small * PA_SMALL * (int64_t)sizeof(float2));
+    p.ml_big = take(p.slots_big * PA_BIG * (int64_t)sizeof(float2));
+    p.o_small = take(p.slots_small * PA_SMALL * dim * 4);
+    p.o_big = take(p.slots_big * PA_BIG * dim * 4);
+  }
+  p.bytes = at;
+  return RTENHIP_OK;
+}
+
+template <int DP, int TYPE>
+static void launch_paged(const PagedDesc& d, hipStream_t s) {
+  if (d.grid_small)
+    hipLaunchKernelGGL((decode_kernel<DP, TYPE>), dim3((unsigned)d.grid_small), dim3(PA_THREADS), 0, s, d);
+  if (d.grid_big)
+    hipLaunchKernelGGL((chunk_kernel<DP, TYPE>), dim3((unsigned)d.grid_big), dim3(PA_THREADS), 0, s, d);
+}
+
+template <int TYPE>
+static void launch_paged(const PagedDesc& d, hipStream_t s) {
+  if (d.c.dim <= 64) launch_paged<64, TYPE>(d, s);
+  else if (d.c.dim <= 128) launch_paged<128, TYPE>(d, s);
+  else launch_paged<256, TYPE>(d, s);
+}
+
+}  // namespace rtenhip
+
+using namespace rtenhip;
+
+extern "C" rtenhip_status rtenhip_paged_attention_workspace(const rtenhip_tensor* q, const rtenhip_kv_cache* cache,
+                                                            const rtenhip_sequences* seqs, size_t* bytes) {
+  if (!bytes) return fail(RTENHIP_MISSING_INPUTS, "Missing output");
+  PagedDesc d{};
+  PagedPlan p;
+  int dtype;
+  const rtenhip_status st = paged_plan(q, cache, seqs, d, dtype, p);
+  if (!st) *bytes = p.bytes;
+  return st;
+}
+
+extern "C" rtenhip_status rtenhip_paged_attention_f32(rtenhip_ctx* ctx, const rtenhip_tensor* q,
+                                                      const rtenhip_kv_cache* cache, const rtenhip_sequences* seqs,
+                                                      float scale, int32_t window, int32_t sinks, void* workspace,
+                                                      size_t workspace_bytes, rtenhip_tensor* out) {
+  PagedDesc d{};
+  PagedPlan p;
+  int dtype;
+  rtenhip_status st = paged_plan(q, cache, seqs, d, dtype, p);
+  if (!st)
+    st = check_rows(out, q->shape[0], q->shape[1], q->shape[2], "out must have the shape of q",
+                    "Head rows must have unit stride and start on 16 bytes");
+  if (st) return st;
+  if (window < 0 || sinks < 0) return fail(RTENHIP_INVALID_VALUE, "window and sinks must not be negative");
+  if (!std::isfinite(scale)) return fail(RTENHIP_INVALID_VALUE, "scale must be finite");
+  if (!rows_apart(out->shape, out->strides, 2, q->shape[2]))
+    return fail(RTENHIP_INVALID_VALUE, "Output rows must not overlap");
+  if (rows_clash(q, out)) return fail(RTENHIP_INVALID_VALUE, "Outputs may share memory with their own input only");
+  if (p.bytes && (!workspace || workspace_bytes < p.bytes))
+    return fail(RTENHIP_INVALID_VALUE, "Workspace is too small");
+  if ((uintptr_t)workspace % 16) return fail(RTENHIP_UNSUPPORTED_VALUE, "Workspace must be on 16 bytes");
+  if (!ctx) return fail(RTENHIP_MISSING_INPUTS, "Missing context");
+  if (!p.grid_small && !p.grid_big) return RTENHIP_OK;
+  d.q = q->data, d.q_t = q->strides[0], d.q_h = q->strides[1];
+  d.out = out->data, d.o_t = out->strides[0], d.o_h = out->strides[1];
+  d.window = window;
+  d.sinks = window ? sinks : 0;
+  d.scale_log2e = scale * 1.44269504088896340736f;
+  d.minus1 = -1.f;
+  d.grid_small = (int)p.grid_small, d.grid_big = (int)p.grid_big;
+  d.slots_small = (int)p.slots_small, d.slots_big = (int)p.slots_big;
+  d.target_small = PA_TARGET_SMALL, d.target_big = PA_TARGET_BIG;
+  char* ws = (char*)workspace;
+  if (p.bytes) {
+    d.part_small = (Part*)(ws + p.part_small);
+    d.part_big = (Part*)(ws + p.part_big);
+    d.ml_small = (float2*)(ws + p.ml_small);
+    d.ml_big = (float2*)(ws + p.ml_big);
+    d.o_small = (float*)(ws + p.o_small);
+    d.o_big = (float*)(ws + p.o_big);
+  }
+  DeviceScope on(reinterpret_cast<Ctx*>(ctx)->device);
+  if (on.status) return on.status;
+  hipStream_t s = stream_of(ctx);
+  if (dtype == RTENHIP_CACHE_F32) launch_paged<RTENHIP_CACHE_F32>(d, s);
+  else if (dtype == RTENHIP_CACHE_F16) launch_paged<RTENHIP_CACHE_F16>(d, s);
+  else launch_paged<RTENHIP_CACHE_BF16>(d, s);
+  RTENHIP_LAUNCH_CHECK();
+  if (p.slots_small) hipLaunchKernelGGL((merge_kernel<false>), dim3((unsigned)p.grid_small), dim3(PA_THREADS), 0, s, d);
+  if (p.slots_big) hipLaunchKernelGGL((merge_kernel<true>), dim3((unsigned)p.grid_big), dim3(PA_THREADS), 0, s, d);
+  RTENHIP_LAUNCH_CHECK();
+  return RTENHIP_OK;
+}

@@ -126,6 +126,8 @@ EXPORTED_SYMBOLS = [
     "rtenhip_set_exec_stream", "rtenhip_host_alloc", "rtenhip_host_free", "rtenhip_graph_run_host", "rtenhip_graph_wait",
     "rtenhip_sharded_create", "rtenhip_sharded_destroy", "rtenhip_sharded_gather_mode",
     "rtenhip_sharded_graph", "rtenhip_sharded_run_host", "rtenhip_sharded_gathered",
+    "rtenhip_qk_norm_rotary_f32", "rtenhip_qk_norm_rotary_append_f32", "rtenhip_paged_attention_workspace",
+    "rtenhip_paged_attention_f32", "rtenhip_sample_workspace", "rtenhip_sample_f32",
 ]
 
 # rtenhip_dtype (sg::DataType order, include/rten_hip.h)
@@ -188,6 +190,7 @@ class Context:
     def sync_stream(self, stream=None):
         torch = _torch()
         s = stream if stream is not None else torch.cuda.current_stream(self.device)
+        self.stream = s
         check(lib().rtenhip_set_stream(C.c_void_p(self.ptr), C.c_void_p(s.cuda_stream)))
 
     def use_stream(self, stream):
@@ -642,3 +645,8 @@ def mul(a, b, **kw):
 
 def div(a, b, **kw):
     return binary("Div", a, b, **kw)
+
+
+# Operators of a decoder (norm and rotation, attention over a paged cache,
+# sampling); imported last: they use the names above.
+from .decoder import paged_attention, qk_norm_rotary, qk_norm_rotary_append, sample  # noqa: E402,F401

@@ -1,0 +1,250 @@
+"""Operators of a decoder that answers token by token (the "decoder operators"
+of include/rten_hip.h): the norm and rotation of queries and keys, attention
+over a paged cache, and sampling.
+
+A cache is a pair of device tensors ``[pages, page size, heads, head_dim]``
+(float32, float16 or bfloat16, any order of the first three dimensions in
+memory, e.g. a transposed ``[pages, heads, page size, head_dim]``).  Sequence s
+owns the pages in row s of ``page_table`` (int32, -1 = none) and has
+``kv_lens[s]`` tokens there.  The rows of a call are the new tokens of its
+sequences, one after the other: ``q_starts[s]`` .. ``q_starts[s + 1]`` - 1 for
+sequence s; without ``q_starts`` row s is the one new token of sequence s.
+Rows from ``q_starts[-1]`` on are padding and left as they are.  ``kv_lens``
+counts the new tokens: append before attending.  All calls only queue work on
+the context's stream and can be captured.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+from . import OpError, Tensor, _torch, check, default_context, lib
+
+CACHE_DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+
+
+class KVCache(C.Structure):
+    """rtenhip_kv_cache."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int32), ("page_size", C.c_int32),
+                ("n_pages", C.c_int64), ("n_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("k_strides", C.c_int64 * 3), ("v_strides", C.c_int64 * 3)]
+
+
+class Sequences(C.Structure):
+    """rtenhip_sequences."""
+    _fields_ = [("page_table", C.c_void_p), ("table_stride", C.c_int64), ("kv_lens", C.c_void_p),
+                ("q_starts", C.c_void_p), ("n_seqs", C.c_int32), ("max_pages", C.c_int32)]
+
+
+class Rotary(C.Structure):
+    """rtenhip_rotary."""
+    _fields_ = [("q_scale", C.c_void_p), ("k_scale", C.c_void_p), ("inv_freq", C.c_void_p),
+                ("positions", C.c_void_p), ("epsilon", C.c_float), ("rotary_dim", C.c_int32),
+                ("interleaved", C.c_int32)]
+
+
+class Sampling(C.Structure):
+    """rtenhip_sampling."""
+    _fields_ = [("temperature", C.c_float), ("top_p", C.c_float), ("min_p", C.c_float), ("top_k", C.c_int32),
+                ("temperatures", C.c_void_p), ("top_ps", C.c_void_p), ("min_ps", C.c_void_p),
+                ("top_ks", C.c_void_p)]
+
+
+_P = C.c_void_p
+_SIGNATURES = {
+    "rtenhip_qk_norm_rotary_f32": [_P] * 6,
+    "rtenhip_qk_norm_rotary_append_f32": [_P] * 8,
+    "rtenhip_paged_attention_workspace": [_P] * 4,
+    "rtenhip_paged_attention_f32": [_P, _P, _P, _P, C.c_float, C.c_int32, C.c_int32, _P, C.c_size_t, _P],
+    "rtenhip_sample_workspace": [C.c_int64, C.c_int64, _P],
+    "rtenhip_sample_f32": [_P, _P, _P, _P, _P, C.c_size_t, _P, _P],
+}
+_functions = {}
+
+
+def _call(name, *args):
+    f = _functions.get(name)
+    if f is None:
+        f = getattr(lib(), name)
+        f.argtypes, f.restype = _SIGNATURES[name], C.c_int
+        _functions[name] = f
+    check(f(*args))
+
+
+def _on_device(t, ctx, dtype, what):
+    if t.dtype != dtype:
+        raise OpError(1, f"IncorrectInputType: expected {str(dtype)[6:]} {what}")
+    if t.get_device() != ctx.device:
+        raise OpError(1, f"{what} must be on the context's GPU")
+
+
+def _rows(t, ctx, what):
+    """rtenhip_tensor of a float32 [tokens, heads, head_dim] (or [rows, vocab]) tensor."""
+    _on_device(t, ctx, _torch().float32, what)
+    if t.dim() > 8:
+        raise OpError(6, "too many dims")
+    return Tensor(t.data_ptr() if t.numel() else None, t.dim(), tuple(t.shape), tuple(t.stride()))
+
+
+def _vector(t, n, ctx, dtype, what):
+    """Address of a contiguous 1-D device tensor of n elements (None: NULL)."""
+    if t is None:
+        return None
+    _on_device(t, ctx, dtype, what)
+    if t.dim() != 1 or t.shape[0] != n:
+        raise OpError(3, f"{what} must have {n} elements")
+    if n > 1 and t.stride(0) != 1:
+        raise OpError(6, f"{what} must be contiguous")
+    return t.data_ptr()
+
+
+def _cache(k, v, ctx):
+    if k.dim() != 4 or k.shape != v.shape:
+        raise OpError(3, "Caches must be [pages, page size, heads, head_dim] of the same shape")
+    if str(k.dtype) not in CACHE_DTYPES:
+        raise OpError(1, "IncorrectInputType: cache must be float32, float16 or bfloat16")
+    _on_device(k, ctx, k.dtype, "cache")
+    _on_device(v, ctx, k.dtype, "cache")
+    n, page, heads, dim = k.shape
+    ks, vs = k.stride(), v.stride()
+    if dim > 1 and (ks[3] != 1 or vs[3] != 1):
+        raise OpError(6, "Cache rows must have unit stride")
+    if page > 65536:
+        raise OpError(5, "Invalid cache size")
+    return KVCache(k.data_ptr() if n else None, v.data_ptr() if n else None, CACHE_DTYPES[str(k.dtype)], page, n, heads,
+                   dim, ks[:3], vs[:3])
+
+
+def _sequences(page_table, kv_lens, q_starts, ctx):
+    i32 = _torch().int32
+    _on_device(page_table, ctx, i32, "page_table")
+    if page_table.dim() != 2:
+        raise OpError(3, "page_table must be [sequences, pages]")
+    n, pages = page_table.shape
+    if pages > 1 and page_table.stride(1) != 1:
+        raise OpError(6, "page_table rows must have unit stride")
+    return Sequences(page_table.data_ptr() if n * pages else None, page_table.stride(0),
+                     _vector(kv_lens, n, ctx, i32, "kv_lens"), _vector(q_starts, n + 1, ctx, i32, "q_starts"), n, pages)
+
+
+def _empty(shape, dtype, ctx):
+    """A tensor whose memory belongs to the context's stream, which is the one
+    that the call writes it on."""
+    torch = _torch()
+    device = torch.device("cuda", ctx.device)
+    if ctx.stream.cuda_stream == torch.cuda.current_stream(ctx.device).cuda_stream:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(ctx.stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _rotary(inv_freq, positions, tokens, dim, q_scale, k_scale, epsilon, interleaved, ctx):
+    torch = _torch()
+    f32 = torch.float32
+    half = 0 if inv_freq is None else inv_freq.shape[0] if inv_freq.dim() == 1 else -1
+    if half < 0:
+        raise OpError(3, "inv_freq must be 1-D")
+    return Rotary(_vector(q_scale, dim, ctx, f32, "q_scale"), _vector(k_scale, dim, ctx, f32, "k_scale"),
+                  _vector(inv_freq, half, ctx, f32, "inv_freq"),
+                  _vector(positions, tokens, ctx, torch.int32, "positions"), epsilon, 2 * half, int(bool(interleaved)))
+
+
+def _check_3d(*tensors):
+    for t in tensors:
+        if t.dim() != 3:
+            raise OpError(3, "Expected [tokens, heads, head_dim] inputs")
+
+
+def qk_norm_rotary(q, k, positions, inv_freq, q_scale=None, k_scale=None, epsilon=1e-6, interleaved=False, q_out=None,
+                   k_out=None, ctx=None):
+    """RMS norm over head_dim (where a scale ``[head_dim]`` is given), then the
+    rotation by ``positions[t] * inv_freq[i]``, of the head rows of q
+    ``[tokens, q heads, head_dim]`` and k ``[tokens, k heads, head_dim]``.
+    ``inv_freq`` has rotary_dim / 2 values (None: no rotation); pairs are
+    (i, i + rotary_dim / 2), or neighbours if ``interleaved``.  Returns
+    (q_out, k_out); either may be given, its input itself included."""
+    ctx = ctx or default_context()
+    _check_3d(q, k)
+    r = _rotary(inv_freq, positions, q.shape[0], q.shape[2], q_scale, k_scale, epsilon, interleaved, ctx)
+    if q_out is None:
+        q_out = _empty(q.shape, q.dtype, ctx)
+    if k_out is None:
+        k_out = _empty(k.shape, k.dtype, ctx)
+    qd, kd, qo, ko = _rows(q, ctx, "q"), _rows(k, ctx, "k"), _rows(q_out, ctx, "q_out"), _rows(k_out, ctx, "k_out")
+    _call("rtenhip_qk_norm_rotary_f32", ctx.ptr, C.byref(qd), C.byref(kd), C.byref(r), C.byref(qo), C.byref(ko))
+    return q_out, k_out
+
+
+def qk_norm_rotary_append(q, k, v, inv_freq, k_cache, v_cache, page_table, kv_lens, q_starts=None, positions=None,
+                          q_scale=None, k_scale=None, epsilon=1e-6, interleaved=False, out=None, ctx=None):
+    """:func:`qk_norm_rotary` of the new tokens of the sequences, with k's rows
+    and v written into the cache.  ``positions`` (default: the tokens' places
+    in their sequences) turn the rows only.  Returns q's rows (``out``, which
+    may be q); rows of padding in a new ``out`` are not initialised."""
+    ctx = ctx or default_context()
+    _check_3d(q, k, v)
+    r = _rotary(inv_freq, positions, q.shape[0], q.shape[2], q_scale, k_scale, epsilon, interleaved, ctx)
+    cache = _cache(k_cache, v_cache, ctx)
+    seqs = _sequences(page_table, kv_lens, q_starts, ctx)
+    if out is None:
+        out = _empty(q.shape, q.dtype, ctx)
+    qd, kd, vd, od = _rows(q, ctx, "q"), _rows(k, ctx, "k"), _rows(v, ctx, "v"), _rows(out, ctx, "out")
+    _call("rtenhip_qk_norm_rotary_append_f32", ctx.ptr, C.byref(qd), C.byref(kd), C.byref(vd), C.byref(r),
+          C.byref(cache), C.byref(seqs), C.byref(od))
+    return out
+
+
+def paged_attention(q, k_cache, v_cache, page_table, kv_lens, q_starts=None, scale=None, window=0, sinks=0, out=None,
+                    ctx=None):
+    """softmax(scale q k^T) v of the new tokens' queries ``[tokens, q heads,
+    head_dim]`` over their sequences' cached tokens; query head h reads cache
+    head h // (q heads / cache heads).  The token at position p sees the tokens
+    up to p; with a ``window``, the last ``window`` of them and the first
+    ``sinks``.  ``scale`` defaults to 1 / sqrt(head_dim).  A row that sees
+    nothing gives zeros; rows of padding in a new ``out`` are not initialised."""
+    ctx = ctx or default_context()
+    cache = _cache(k_cache, v_cache, ctx)
+    seqs = _sequences(page_table, kv_lens, q_starts, ctx)
+    qd = _rows(q, ctx, "q")
+    if out is None:
+        out = _empty(q.shape, q.dtype, ctx)
+    od = _rows(out, ctx, "out")
+    need = C.c_size_t()
+    _call("rtenhip_paged_attention_workspace", C.byref(qd), C.byref(cache), C.byref(seqs), C.byref(need))
+    n = need.value
+    ws = _empty((n,), _torch().uint8, ctx) if n else None
+    _call("rtenhip_paged_attention_f32", ctx.ptr, C.byref(qd), C.byref(cache), C.byref(seqs),
+          1 / math.sqrt(cache.head_dim) if scale is None else scale, window, sinks, ws.data_ptr() if n else None, n,
+          C.byref(od))
+    return out
+
+
+def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ctx=None):
+    """One token of each row of ``logits [rows, vocab]`` by the random numbers
+    ``uniforms [rows]`` in [0, 1); returns (tokens int32 [rows], logprobs
+    float32 [rows]).  The filters (see rtenhip_sample_f32; ``top_k`` 0,
+    ``top_p`` 1 and ``min_p`` 0 keep all, ``temperature`` 0 takes the largest)
+    are numbers, or device tensors with one for each row."""
+    torch = _torch()
+    ctx = ctx or default_context()
+    ld = _rows(logits, ctx, "logits")
+    if logits.dim() != 2:
+        raise OpError(3, "Expected [rows, vocab] logits")
+    rows, vocab = logits.shape
+    s = Sampling(1.0, 1.0, 0.0, 0)
+    for name, value in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p), ("top_k", top_k)):
+        if isinstance(value, torch.Tensor):
+            dtype = torch.int32 if name == "top_k" else torch.float32
+            setattr(s, name + "s", _vector(value, rows, ctx, dtype, name))
+        elif name == "top_k":
+            s.top_k = min(max(int(value), 0), vocab)
+        else:
+            setattr(s, name, value)
+    u = _vector(uniforms, rows, ctx, torch.float32, "uniforms")
+    tokens, logprobs = _empty((rows,), torch.int32, ctx), _empty((rows,), torch.float32, ctx)
+    need = C.c_size_t()
+    _call("rtenhip_sample_workspace", rows, vocab, C.byref(need))
+    ws = _empty((need.value,), torch.uint8, ctx)
+    _call("rtenhip_sample_f32", ctx.ptr, C.byref(ld), C.byref(s), u, ws.data_ptr(), need.value, tokens.data_ptr(),
+          logprobs.data_ptr())
+    return tokens, logprobs
