@@ -9,8 +9,8 @@
 //
 // A sequence with at most 16 rows (new tokens x heads of a group) runs in
 // decode_kernel, where the cache streams from memory straight into the
-// registers of the matrix instructions; the others run in chunk_kernel, 128
-// rows a workgroup, where a tile of 64 keys and values is shared through LDS.
+// registers of the matrix instructions; the others run in chunk_kernel, up to
+// 256 rows a workgroup, where tiles of keys and values are shared through LDS.
 // Lengths live on the device, so each workgroup finds its own piece of work
 // (plan): the visible keys of all sequences, counted in tiles of 64, are
 // divided into stretches of about equal length, one to a workgroup.  Where a
@@ -36,7 +36,6 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int PA_THREADS = 256;
 constexpr int PA_UNIT = 64;    // keys of a tile
 constexpr int PA_SMALL = 16;   // rows of a decode tile
-constexpr int PA_BIG = 128;    // rows of a chunk tile
 constexpr float NEG_INF = -__builtin_huge_valf();
 
 // What merge_kernel has to know of a stretch.
@@ -59,25 +58,27 @@ struct PagedDesc {
   int small_only;  // every sequence has at most PA_SMALL rows
   // Workspace: the stretches of the decode grid, then those of the chunk grid.
   int grid_small, grid_big, slots_small, slots_big;
-  int target_small, target_big;
-  Part* part_small;
+  int target_small, target_big, rows_big;
+  int* slots;        // stretches to join: [decode, chunk]
+  Part* part_small;  // [slots]
   Part* part_big;
   float* o_small;  // [slots][PA_SMALL][dim] normalised results
-  float* o_big;    // [slots][PA_BIG][dim]
+  float* o_big;    // [slots][rows of a chunk tile][dim]
   float2* ml_small;  // [slots][PA_SMALL] (m, l)
   float2* ml_big;
 };
 
 // ---- plan ------------------------------------------------------------------------
 
-// The tiles of 64 keys that positions p0 .. p1 see: `sinks` whole tiles from 0
-// and then those from lo on.
+// The tiles of TN keys that positions p0 .. p1 see: those of the sinks from 0
+// on and then those from lo on.
 struct Span {
   int sink_tiles, lo_tile, tiles;
   int lo, end;  // keys in [0, sinks) and [lo, end) are seen by some row
   __device__ __forceinline__ int tile(int i) const { return i < sink_tiles ? i : i - sink_tiles + lo_tile; }
 };
 
+template <int TN>
 __device__ __forceinline__ Span span_of(const PagedDesc& d, int kv_len, int p0, int p1) {
   Span v;
   // (A tile's last key stays below 2^31.)
@@ -90,11 +91,11 @@ __device__ __forceinline__ Span span_of(const PagedDesc& d, int kv_len, int p0, 
   if (d.window) {
     const int64_t lo = (int64_t)p0 - d.window + 1;
     v.lo = lo < 0 ? 0 : (int)lo;
-    v.lo_tile = v.lo / PA_UNIT;
-    v.sink_tiles = min((min(d.sinks, v.end) + PA_UNIT - 1) / PA_UNIT, v.lo_tile);
+    v.lo_tile = v.lo / TN;
+    v.sink_tiles = min((min(d.sinks, v.end) + TN - 1) / TN, v.lo_tile);
   }
-  v.lo_tile = v.lo / PA_UNIT;
-  v.tiles = v.sink_tiles + max(0, (v.end + PA_UNIT - 1) / PA_UNIT - v.lo_tile);
+  v.lo_tile = v.lo / TN;
+  v.tiles = v.sink_tiles + max(0, (v.end + TN - 1) / TN - v.lo_tile);
   return v;
 }
 
@@ -107,7 +108,7 @@ struct SeqWork {
   int start, q_len, kv_len, tiles, units;  // tiles of rows, tiles of keys
 };
 
-template <bool BIG>
+template <bool BIG, int ROWS>
 __device__ __forceinline__ SeqWork seq_work(const PagedDesc& d, int s) {
   SeqWork w;
   w.start = seq_start(d.s, s);
@@ -116,16 +117,16 @@ __device__ __forceinline__ SeqWork seq_work(const PagedDesc& d, int s) {
   const int64_t rows = (int64_t)w.q_len * d.group;
   w.units = 0;
   if (BIG)
-    w.tiles = rows > PA_SMALL ? (int)((rows + PA_BIG - 1) / PA_BIG) : 0;
+    w.tiles = rows > PA_SMALL ? (int)((rows + ROWS - 1) / ROWS) : 0;
   else
     w.tiles = rows > 0 && rows <= PA_SMALL;
-  if (w.tiles) w.units = max(1, span_of(d, w.kv_len, w.kv_len - w.q_len, w.kv_len - 1).tiles);
+  if (w.tiles) w.units = max(1, span_of<PA_UNIT>(d, w.kv_len, w.kv_len - w.q_len, w.kv_len - 1).tiles);
   return w;
 }
 
 struct PlanShared {
-  int64_t units[4];
-  int items[4], slots[4];
+  int64_t units[8];  // of each wave
+  int items[8], slots[8];
   Work work;
 };
 
@@ -142,15 +143,15 @@ __device__ __forceinline__ int wave_scan(int x) {  // inclusive
 // The piece of work of workgroup `block`: false if there is none.  Every
 // workgroup counts for itself (thread i the sequences i * each ..), which
 // costs no launch and no order between workgroups.
-template <bool BIG>
+template <bool BIG, int THREADS, int ROWS>
 __device__ bool plan(const PagedDesc& d, int block, PlanShared& sh, Work& out) {
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const int each = (d.s.n + PA_THREADS - 1) / PA_THREADS;
+  const int each = (d.s.n + THREADS - 1) / THREADS;
   const int s0 = tid * each, s1 = min(d.s.n, s0 + each);
   const int heads = d.c.heads;
   int64_t units = 0;
   for (int s = s0; s < s1; s++) {
-    const SeqWork w = seq_work<BIG>(d, s);
+    const SeqWork w = seq_work<BIG, ROWS>(d, s);
     units += (int64_t)w.tiles * w.units;
   }
 #pragma unroll
@@ -158,7 +159,9 @@ __device__ bool plan(const PagedDesc& d, int block, PlanShared& sh, Work& out) {
   if (lane == 0) sh.units[wave] = units;
   if (tid == 0) sh.work.seq = -1;
   __syncthreads();
-  const int64_t total = (sh.units[0] + sh.units[1] + sh.units[2] + sh.units[3]) * heads;
+  int64_t total = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; i++) total += sh.units[i] * heads;
   const int64_t target = BIG ? d.target_big : d.target_small;
   // Keys of a stretch, in tiles: stretches for the whole card, none shorter
   // than a tile.
@@ -166,7 +169,7 @@ __device__ bool plan(const PagedDesc& d, int block, PlanShared& sh, Work& out) {
   const int len = (int)(len64 < 1 ? 1 : len64 > (1 << 26) ? (1 << 26) : len64);
   int items = 0, slots = 0;
   for (int s = s0; s < s1; s++) {
-    const SeqWork w = seq_work<BIG>(d, s);
+    const SeqWork w = seq_work<BIG, ROWS>(d, s);
     const int parts = (w.units + len - 1) / len;
     const int n = w.tiles * heads * parts;
     items += n;
@@ -175,11 +178,17 @@ __device__ bool plan(const PagedDesc& d, int block, PlanShared& sh, Work& out) {
   const int items_in = wave_scan(items), slots_in = wave_scan(slots);
   if (lane == 63) sh.items[wave] = items_in, sh.slots[wave] = slots_in;
   __syncthreads();
+  if (block == 0 && tid == 0 && d.slots) {
+    int n = 0;
+    for (int w = 0; w < THREADS / 64; w++) n += sh.slots[w];
+    d.slots[BIG] = min(n, BIG ? d.slots_big : d.slots_small);
+    if (!(BIG ? d.grid_small : d.grid_big)) d.slots[!BIG] = 0;  // the other kernel does not run
+  }
   int at = items_in - items, slot = slots_in - slots;
   for (int w = 0; w < wave; w++) at += sh.items[w], slot += sh.slots[w];
   if (block >= at && block < at + items) {
     for (int s = s0; s < s1; s++) {
-      const SeqWork w = seq_work<BIG>(d, s);
+      const SeqWork w = seq_work<BIG, ROWS>(d, s);
       const int parts = (w.units + len - 1) / len;
       const int n = w.tiles * heads * parts;
       if (block < at + n) {
@@ -340,14 +349,9 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
   __shared__ float o_sh[4][PA_SMALL][DP];
   __shared__ float m_sh[4][PA_SMALL], l_sh[4][PA_SMALL];
   Work w;
-  const bool any = plan<false>(d, blockIdx.x, plan_sh, w);
-  if (threadIdx.x == 0 && d.part_small) {
-    Part p{};
-    if (any && w.slot >= 0 && w.slot < d.slots_small)
-      p = Part{w.slot, w.part, w.parts, d.c.heads, w.start, 0, w.q_len * d.group, w.head};
-    d.part_small[blockIdx.x] = p;
-  }
-  if (!any || w.slot >= d.slots_small) return;
+  if (!plan<false, PA_THREADS, PA_SMALL>(d, blockIdx.x, plan_sh, w) || w.slot >= d.slots_small) return;
+  if (threadIdx.x == 0 && w.slot >= 0)
+    d.part_small[w.slot] = Part{w.slot, w.part, w.parts, d.c.heads, w.start, 0, w.q_len * d.group, w.head};
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int i = lane & 15, g = lane >> 4;
   const int dim = d.c.dim, rows = w.q_len * d.group;
@@ -414,7 +418,7 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
     }
   }
 
-  const Span span = span_of(d, w.kv_len, w.kv_len - w.q_len, w.kv_len - 1);
+  const Span span = span_of<PA_UNIT>(d, w.kv_len, w.kv_len - w.q_len, w.kv_len - 1);
   const int u0 = (int)((int64_t)span.tiles * w.part / w.parts), u1 = (int)((int64_t)span.tiles * (w.part + 1) / w.parts);
   const int* table = d.s.table + (int64_t)w.seq * d.s.table_stride;
   const char* kc = d.c.k + (int64_t)w.head * d.c.k_head * size;
@@ -628,14 +632,14 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
 
 // ---- chunk ---------------------------------------------------------------------------
 
-// 128 rows (new token, head of the group) a workgroup, 32 a wave.  A tile of
-// 64 keys and values goes to LDS as f16 terms, and both products run on the
-// f16 matrix instructions:
+// 256 rows (new token, head of the group) a workgroup, 32 a wave.  Tiles of
+// keys and values go to LDS as f16 terms, and both products run on the f16
+// matrix instructions:
 //  - an f32 number x 2^e is hi + lo, each f16 (split16), and a product
 //    hi hi + hi lo + lo hi, three f16 instructions against the eight times
 //    longer f32 one, loses what is below 2^-22 of it; a 16-bit cache needs no
 //    lo.  e is one power of two for the tile's keys and one, which only ever
-//    grows, for the values so far, so the largest number of either is near
+//    falls, for the values so far, so the largest number of either is near
 //    2^13 and the terms are exact to 2^-38 of it; q has one for each row, p
 //    the factor 2^8.  Powers of two come out again exactly.
 //  - S^T = K Q^T: a lane (n, h) has row n's scores for the keys
@@ -646,22 +650,39 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
 //  The maximum that p is taken against follows the largest score only when it
 //  is passed by more than 2^6, which few tiles do, so the result is hardly
 //  ever rescaled.
-// Bound by the matrix instructions at long prompts; two workgroups on a CU,
-// so that one's loads, maxima and conversions run under the other's products.
+// Two LDS buffers and one barrier a tile: while tile u is multiplied, u + 1 is
+// converted into the other buffer and u + 2 is on its way into registers.
+// Eight waves, two to a SIMD, so that one's conversions and exponentials run
+// under the other's products; at head_dim 256 a wave needs all of a SIMD's
+// registers, and four waves work on tiles of 32 keys.
+// Bound by the matrix instructions at long prompts.
 template <int DP, int TYPE>
 struct ChunkTile {
+  static constexpr int WAVES = DP == 256 ? 4 : 8, THREADS = 64 * WAVES;
+  static constexpr int TN = DP == 256 ? 32 : 64;  // keys of a tile
+  static constexpr int ROWS = 32 * WAVES;
   static constexpr int TERMS = TYPE == RTENHIP_CACHE_F32 ? 2 : 1;
   static constexpr int KS = DP * 2 + 16;  // bytes of a key's row in LDS, off by a bank group per row
-  static constexpr int KL = DP * CacheType<TYPE>::size / 64;          // 16-byte loads of keys per thread
-  static constexpr int VW = DP / 16 * CacheType<TYPE>::size / 4;      // words of values per thread and key
-  static constexpr int K_BYTES = PA_UNIT * KS, V_BYTES = DP * PA_UNIT * 2;
+  static constexpr int KL = DP * CacheType<TYPE>::size / 128;     // 16-byte loads of keys per thread (8 to a row)
+  static constexpr int DPV = DP / 32;                             // value dimensions per thread, of 4 keys
+  static constexpr int VW = DPV * CacheType<TYPE>::size / 4;      // words of values per thread and key
+  static constexpr int K_BYTES = TN * KS, V_BYTES = DP * TN * 2;
+  static constexpr int BUFFER = TERMS * (K_BYTES + V_BYTES);
 };
+
+// Rows of a chunk tile (what the plan counts in).
+template <int DP>
+constexpr int chunk_rows() {
+  return ChunkTile<DP, RTENHIP_CACHE_F32>::ROWS;
+}
 
 // Where the 16 bytes of keys (h, i, j), chunk = 2 * (16 keys) + h, of a
 // dimension lie: the chunks of neighbouring dimensions, and of dimensions 8
 // apart, are in different banks.
+template <int TN>
 __device__ __forceinline__ int value_at(int dimension, int chunk) {
-  return dimension * (PA_UNIT * 2) + ((chunk ^ dimension ^ (dimension >> 3)) & 7) * 16;
+  if constexpr (TN == 64) return dimension * 128 + ((chunk ^ dimension ^ (dimension >> 3)) & 7) * 16;
+  return dimension * 64 + ((chunk ^ (dimension >> 1) ^ (dimension >> 3)) & 3) * 16;
 }
 
 template <int TYPE>
@@ -682,30 +703,44 @@ __device__ __forceinline__ float top_of(float top, uint32_t w) {
   return fmaxf(top, fmaxf(fabsf(cache_lo<TYPE>(w)), fabsf(cache_hi<TYPE>(w))));
 }
 
+template <int WORDS>
+__device__ __forceinline__ void load_words(const char* p, bool ok, uint32_t* v) {
+#pragma unroll
+  for (int c = 0; c < WORDS; c++) v[c] = 0;
+  if (!ok) return;
+  if constexpr (WORDS == 1) {
+    v[0] = *(const uint32_t*)p;
+  } else if constexpr (WORDS == 2) {
+    const u32x2 x = *(const u32x2*)p;
+    v[0] = x[0], v[1] = x[1];
+  } else {
+#pragma unroll
+    for (int c = 0; c < WORDS; c += 4) {
+      const u32x4 x = *(const u32x4*)(p + 4 * c);
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[c + e] = x[e];
+    }
+  }
+}
+
 template <int DP, int TYPE>
-__global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void chunk_kernel(PagedDesc d) {
+__global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) void chunk_kernel(PagedDesc d) {
   using T = ChunkTile<DP, TYPE>;
-  constexpr int TERMS = T::TERMS, KS = T::KS, KL = T::KL, VW = T::VW, DPL = DP / 16;
+  constexpr int TERMS = T::TERMS, KS = T::KS, KL = T::KL, VW = T::VW, DPV = T::DPV, TN = T::TN, WAVES = T::WAVES;
   constexpr int size = CacheType<TYPE>::size, PER = 16 / size, NB = DP / 32;
   constexpr bool SCALED = TYPE != RTENHIP_CACHE_F16;  // f16 rows go to LDS as they are
   __shared__ PlanShared plan_sh;
-  __shared__ __attribute__((aligned(16))) char k_sh[TERMS][T::K_BYTES];
-  __shared__ __attribute__((aligned(16))) char v_sh[TERMS][T::V_BYTES];
-  __shared__ float top_sh[2][4];
-  __shared__ int hole_sh[4];
-  __shared__ __attribute__((aligned(4))) uint8_t seen_sh[PA_UNIT], bad_sh[PA_UNIT];
+  __shared__ __attribute__((aligned(16))) char buffer_sh[2][T::BUFFER];  // keys hi, lo, values hi, lo
+  __shared__ float top_sh[2][2][WAVES];                                  // [tile & 1][keys, values]
+  __shared__ int hole_sh[2][WAVES];
+  __shared__ __attribute__((aligned(4))) uint8_t seen_sh[4][TN], bad_sh[4][TN];  // [tile & 3]: read late
   Work w;
-  const bool any = plan<true>(d, blockIdx.x, plan_sh, w);
-  const int row0 = w.tile * PA_BIG;
-  const int all_rows = any ? w.q_len * d.group : 0;
-  const int rows = min(PA_BIG, all_rows - row0);
-  if (threadIdx.x == 0 && d.part_big) {
-    Part p{};
-    if (any && w.slot >= 0 && w.slot < d.slots_big)
-      p = Part{w.slot, w.part, w.parts, d.c.heads, w.start, row0, rows, w.head};
-    d.part_big[blockIdx.x] = p;
-  }
-  if (!any || w.slot >= d.slots_big) return;
+  if (!plan<true, T::THREADS, T::ROWS>(d, blockIdx.x, plan_sh, w) || w.slot >= d.slots_big) return;
+  const int row0 = w.tile * T::ROWS;
+  const int all_rows = w.q_len * d.group;
+  const int rows = min(T::ROWS, all_rows - row0);
+  if (threadIdx.x == 0 && w.slot >= 0)
+    d.part_big[w.slot] = Part{w.slot, w.part, w.parts, d.c.heads, w.start, row0, rows, w.head};
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int n = lane & 31, h = lane >> 5;
   const int dim = d.c.dim, first = w.kv_len - w.q_len;
@@ -751,20 +786,22 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void chunk_kernel(Pa
       }
   }
 
-  const Span span = span_of(d, w.kv_len, first + fdiv(row0, d.group_div),
-                            first + fdiv(row0 + rows - 1, d.group_div));
+  const Span span = span_of<TN>(d, w.kv_len, first + fdiv(row0, d.group_div),
+                                first + fdiv(row0 + rows - 1, d.group_div));
   const int u0 = (int)((int64_t)span.tiles * w.part / w.parts), u1 = (int)((int64_t)span.tiles * (w.part + 1) / w.parts);
   const int* table = d.s.table + (int64_t)w.seq * d.s.table_stride;
   const char* kc = d.c.k + (int64_t)w.head * d.c.k_head * size;
   const char* vc = d.c.v + (int64_t)w.head * d.c.v_head * size;
 
-  // Staging: keys, thread (row, quarter); values, thread (4 keys, DP / 16
-  // dimensions).
-  const int k_row = tid >> 2, k_quarter = tid & 3, v_four = tid >> 4, v_group = tid & 15;
+  // Staging: keys, thread (row, eighth of it); values, thread (4 keys, DP / 32
+  // dimensions), the two halves of a wave on the two halves of a chunk.
+  const int k_row = tid >> 3, k_eighth = tid & 7, v_group = tid & 31;
+  const int v_chunk = (tid >> 7) * 2 + (tid >> 6 & 1), v_half = tid >> 5 & 1;
+  const int v_key = 16 * (tid >> 7) + 8 * v_half + 4 * (tid >> 6 & 1);
   auto seen_key = [&](int key) { return key < span.end && (key >= span.lo || key < d.sinks); };
   auto page_at = [&](int u, int at) {
     if (u >= u1) return -1;
-    const int key = span.tile(u) * PA_UNIT + at;
+    const int key = span.tile(u) * TN + at;
     return seen_key(key) ? page_of(table, d.s.max_pages, d.c, key) : -1;
   };
   auto slot_of = [&](int key) { return key - fdiv(key, d.c.page_div) * d.c.page_size; };
@@ -774,34 +811,219 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void chunk_kernel(Pa
   auto find_pages = [&](int u) {
     k_page = page_at(u, k_row);
 #pragma unroll
-    for (int r = 0; r < 4; r++) v_page[r] = page_at(u, 4 * v_four + r);
+    for (int r = 0; r < 4; r++) v_page[r] = page_at(u, v_key + r);
   };
-  bool k_here, k_hole;  // the row in flight: a key somebody sees; one that would be seen but has no page
+  // The row in flight: a key that somebody sees; one that would be seen but
+  // has no page.
+  bool k_here, k_hole;
   auto load = [&](int u) {
-    const int base = u < u1 ? span.tile(u) * PA_UNIT : 0;
+    const int base = u < u1 ? span.tile(u) * TN : 0;
     k_here = k_page >= 0;
     k_hole = u < u1 && !k_here && seen_key(base + k_row);
     const char* kr = kc + ((int64_t)k_page * d.c.k_page + (int64_t)slot_of(base + k_row) * d.c.k_slot) * size;
 #pragma unroll
     for (int j = 0; j < KL; j++) {
-      const int at = (4 * j + k_quarter) * PER;
+      const int at = (8 * j + k_eighth) * PER;
       k_in[j] = (u32x4){0, 0, 0, 0};
       if (k_here && at < dim) k_in[j] = *(const u32x4*)(kr + at * size);
     }
 #pragma unroll
-    for (int r = 0; r < 4; r++)
-      load_values<DP, TYPE>(
-          vc + ((int64_t)v_page[r] * d.c.v_page + (int64_t)slot_of(base + 4 * v_four + r) * d.c.v_slot) * size,
-          v_page[r] >= 0, v_group, dim, v_in[r]);
+    for (int r = 0; r < 4; r++) {
+      const char* vr = vc + ((int64_t)v_page[r] * d.c.v_page + (int64_t)slot_of(base + v_key + r) * d.c.v_slot) * size;
+      load_words<VW>(vr + v_group * DPV * size, v_page[r] >= 0 && v_group * DPV < dim, v_in[r]);
+    }
+  };
+  // What the conversion of the tile in the registers has to know of all of it.
+  auto measure = [&](int u, bool careful) {
+    const int parity = u & 1;
+    if (careful) {
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        bool bad = false;
+#pragma unroll
+        for (int c = 0; c < VW; c++) bad |= clean<TYPE>(v_in[r][c]);
+        const uint64_t all = __ballot(bad);  // (a key's values are in one half of the wave)
+        if (v_group == 0) bad_sh[u & 3][v_key + r] = (uint32_t)(all >> (lane & 32)) != 0;
+      }
+    }
+    if constexpr (SCALED) {
+      float k_top = 0.f, v_top = 0.f;
+#pragma unroll
+      for (int j = 0; j < KL; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          uint32_t x = k_in[j][e];
+          if (careful) clean<TYPE>(x);
+          k_top = top_of<TYPE>(k_top, x);
+        }
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int c = 0; c < VW; c++) v_top = top_of<TYPE>(v_top, v_in[r][c]);
+      k_top = wave_max(k_top);
+      v_top = wave_max(v_top);
+      if (lane == 0) top_sh[parity][0][wave] = k_top, top_sh[parity][1][wave] = v_top;
+    }
+    const bool hole = __any(k_hole);
+    if (lane == 0) hole_sh[parity][wave] = hole;
+    if (k_eighth == 0) seen_sh[u & 3][k_row] = k_here;
   };
 
   float m, l;
   f32x16 o[NB];
-  int v_up;
-  bool poison;
+  int o_up;                         // o is 2^o_up times the result
+  int k_up = 0, v_up;               // exponents of the tile converted last
+  bool holes = false, poison;
+  // Converts the tile in the registers into its buffer.
+  auto stage = [&](int parity) {
+    float k_f = 1.f, v_f = 1.f;
+    if constexpr (SCALED) {
+      float k_top = 0.f, v_top = 0.f;
+#pragma unroll
+      for (int i = 0; i < WAVES; i++)
+        k_top = fmaxf(k_top, top_sh[parity][0][i]), v_top = fmaxf(v_top, top_sh[parity][1][i]);
+      k_up = exponent_for(k_top);
+      const int up = exponent_for(v_top);
+      if (up < v_up) v_up = up - 1;  // larger values than any before: a binade more of room
+      k_f = pow2(k_up);
+      v_f = pow2(v_up);
+    }
+    holes = false;
+#pragma unroll
+    for (int i = 0; i < WAVES; i++) holes |= hole_sh[parity][i] != 0;
+    char* kt = &buffer_sh[parity][k_row * KS];
+#pragma unroll
+    for (int j = 0; j < KL; j++) {
+      const int at = (8 * j + k_eighth) * PER * 2;
+      if constexpr (TYPE == RTENHIP_CACHE_F16) {
+        *(u32x4*)(kt + at) = k_in[j];
+      } else if constexpr (TYPE == RTENHIP_CACHE_BF16) {
+        u32x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          y[e] = __builtin_bit_cast(uint32_t, (f16x2){(_Float16)(cache_lo<TYPE>(k_in[j][e]) * k_f),
+                                                      (_Float16)(cache_hi<TYPE>(k_in[j][e]) * k_f)});
+        *(u32x4*)(kt + at) = y;
+      } else {
+        f16x2 h0, l0, h1, l1;
+        split16(__uint_as_float(k_in[j][0]) * k_f, __uint_as_float(k_in[j][1]) * k_f, d.minus1, h0, l0);
+        split16(__uint_as_float(k_in[j][2]) * k_f, __uint_as_float(k_in[j][3]) * k_f, d.minus1, h1, l1);
+        *(f16x4*)(kt + at) = (f16x4){h0[0], h0[1], h1[0], h1[1]};
+        *(f16x4*)(kt + T::K_BYTES + at) = (f16x4){l0[0], l0[1], l1[0], l1[1]};
+      }
+    }
+    char* vt = &buffer_sh[parity][TERMS * T::K_BYTES + 8 * v_half];
+#pragma unroll
+    for (int e = 0; e < DPV; e++) {
+      const int at = value_at<TN>(DPV * v_group + e, v_chunk);
+      if constexpr (TYPE == RTENHIP_CACHE_F16) {
+        const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+        *(u32x2*)(vt + at) = (u32x2){__builtin_amdgcn_perm(v_in[1][e / 2], v_in[0][e / 2], sel),
+                                     __builtin_amdgcn_perm(v_in[3][e / 2], v_in[2][e / 2], sel)};
+      } else if constexpr (TYPE == RTENHIP_CACHE_BF16) {
+        float x[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          x[r] = (e & 1 ? cache_hi<TYPE>(v_in[r][e / 2]) : cache_lo<TYPE>(v_in[r][e / 2])) * v_f;
+        *(f16x4*)(vt + at) = (f16x4){(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+      } else {
+        f16x2 h0, l0, h1, l1;
+        split16(__uint_as_float(v_in[0][e]) * v_f, __uint_as_float(v_in[1][e]) * v_f, d.minus1, h0, l0);
+        split16(__uint_as_float(v_in[2][e]) * v_f, __uint_as_float(v_in[3][e]) * v_f, d.minus1, h1, l1);
+        *(f16x4*)(vt + at) = (f16x4){h0[0], h0[1], h1[0], h1[1]};
+        *(f16x4*)(vt + T::V_BYTES + at) = (f16x4){l0[0], l0[1], l1[0], l1[1]};
+      }
+    }
+  };
+  auto multiply = [&](int u, int k_exp, bool some_hole, bool careful) {
+    const int base = span.tile(u) * TN, parity = u & 1;
+    // Tiles past all of the wave's rows, or before all their windows.
+    const int64_t below_lo = d.window ? (int64_t)pos_lo - d.window : -1;
+    if (!wave_ok || base > pos_hi || (d.window && base + TN - 1 <= below_lo && base >= d.sinks)) return;
+    const int64_t below_hi = d.window ? (int64_t)pos_hi - d.window : -1;
+    const bool whole = !some_hole && !careful && wave_row + 31 < all_rows && base + TN - 1 <= pos_lo &&
+                       base + TN <= span.end && (base > below_hi || base + TN <= d.sinks);
+    const float back = pow2(-q_up - k_exp);
+    const char* ks = buffer_sh[parity];
+    const char* vs = ks + TERMS * T::K_BYTES;
+#pragma unroll 1
+    for (int tb = 0; tb < TN / 32; tb++) {
+      f32x16 s;
+#pragma unroll
+      for (int e = 0; e < 16; e++) s[e] = 0.f;
+      const char* kr = ks + (32 * tb + n) * KS + 16 * h;
+#pragma unroll
+      for (int j = 0; j < DP / 16; j++) {
+        const f16x8 a = *(const f16x8*)(kr + 32 * j);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q_hi[j], s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q_lo[j], s, 0, 0, 0);
+        if constexpr (TERMS == 2) {
+          const f16x8 b = *(const f16x8*)(kr + T::K_BYTES + 32 * j);
+          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, q_hi[j], s, 0, 0, 0);
+        }
+      }
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const int in = 32 * tb + 2 * e + 4 * h, at = base + in;
+          const uint32_t here = *(const uint32_t*)&seen_sh[u & 3][in];
+          const uint32_t bad = careful ? *(const uint32_t*)&bad_sh[u & 3][in] : 0;
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const bool seen = (here >> (8 * r) & 1) && at + r <= pos && (at + r > below || at + r < d.sinks);
+            if (!seen) s[e + r] = NEG_INF;
+            poison |= seen && (bad >> (8 * r) & 1);
+          }
+        }
+      }
+      float top = s[0];
+#pragma unroll
+      for (int e = 1; e < 16; e++) top = fmaxf(top, s[e]);
+      top = half_max(top) * back;
+      if (__any(top > m + 6.f)) {
+        const float m_new = fmaxf(m, top);
+        const float fade = __builtin_amdgcn_exp2f(m - (m_new == NEG_INF ? 0.f : m_new));
+        m = m_new;
+        l *= fade;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int e = 0; e < 16; e++) o[b][e] *= fade;
+      }
+      // p 2^8: at most 2^14.
+      const float ref = 8.f - (m == NEG_INF ? 0.f : m);
+      f16x8 p_hi[2], p_lo[2];
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; e += 2) {
+        const float a = __builtin_amdgcn_exp2f(__fmaf_rn(s[e], back, ref));
+        const float b = __builtin_amdgcn_exp2f(__fmaf_rn(s[e + 1], back, ref));
+        sum += a + b;
+        f16x2 hi, lo;
+        split16(a, b, d.minus1, hi, lo);
+        p_hi[e >> 3][e & 7] = hi[0], p_hi[e >> 3][(e & 7) + 1] = hi[1];
+        p_lo[e >> 3][e & 7] = lo[0], p_lo[e >> 3][(e & 7) + 1] = lo[1];
+      }
+      l += sum;
+#pragma unroll
+      for (int c = 0; c < 2; c++)
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+          const int at = value_at<TN>(32 * b + n, 2 * (2 * tb + c) + h);
+          const f16x8 a = *(const f16x8*)(vs + at);
+          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p_hi[c], o[b], 0, 0, 0);
+          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p_lo[c], o[b], 0, 0, 0);
+          if constexpr (TERMS == 2) {
+            const f16x8 z = *(const f16x8*)(vs + T::V_BYTES + at);
+            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(z, p_hi[c], o[b], 0, 0, 0);
+          }
+        }
+    }
+  };
+  // A tile's buffer, tops and flags go by the parity of its number.
   auto pass = [&](bool careful) {
     m = NEG_INF, l = 0.f;
-    v_up = 113;  // as for values that are all zero or very small
+    o_up = v_up = 113;  // as for values that are all zero or very small
     poison = false;
 #pragma unroll
     for (int b = 0; b < NB; b++)
@@ -810,197 +1032,33 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void chunk_kernel(Pa
     find_pages(u0);
     load(u0);
     find_pages(u0 + 1);
+    measure(u0, careful);
+    __syncthreads();
+    stage(u0 & 1);
+    load(u0 + 1);
+    find_pages(u0 + 2);
+    measure(u0 + 1, careful);
     for (int u = u0; u < u1; u++) {
-      const int base = span.tile(u) * PA_UNIT;
-      bool v_bad[4] = {false, false, false, false};
-      if (careful) {
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-#pragma unroll
-          for (int c = 0; c < VW; c++) v_bad[r] |= clean<TYPE>(v_in[r][c]);
-      }
-      float k_top = 0.f, v_top = 0.f;
-      if constexpr (SCALED) {
-#pragma unroll
-        for (int j = 0; j < KL; j++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            uint32_t x = k_in[j][e];
-            if (careful) clean<TYPE>(x);
-            k_top = top_of<TYPE>(k_top, x);
-          }
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-#pragma unroll
-          for (int c = 0; c < VW; c++) v_top = top_of<TYPE>(v_top, v_in[r][c]);
-        k_top = wave_max(k_top);
-        v_top = wave_max(v_top);
-        if (lane == 0) top_sh[0][wave] = k_top, top_sh[1][wave] = v_top;
-      }
-      const bool hole = __any(k_hole);
-      if (lane == 0) hole_sh[wave] = hole;
-      // Everybody is through with the tile before, and the tops are there.
+      const int k_exp = k_up, v_exp = v_up;
+      const bool some_hole = holes;
+      // Tile u is in its buffer, u + 1's tops are there, and nobody reads
+      // u - 1 any more.
       __syncthreads();
-      int k_up = 0;
-      float v_f = 1.f;
-      if constexpr (SCALED) {
-        k_up = exponent_for(fmaxf(fmaxf(top_sh[0][0], top_sh[0][1]), fmaxf(top_sh[0][2], top_sh[0][3])));
-        const int up = exponent_for(fmaxf(fmaxf(top_sh[1][0], top_sh[1][1]), fmaxf(top_sh[1][2], top_sh[1][3])));
-        if (up < v_up) {  // larger values than any before: one binade of room more
-          const float f = pow2(up - 1 - v_up);
-          v_up = up - 1;
+      if (u + 1 < u1) stage((u + 1) & 1);
+      load(u + 2);
+      find_pages(u + 3);
+      if (SCALED && v_exp != o_up) {
+        const float f = pow2(v_exp - o_up);
+        o_up = v_exp;
 #pragma unroll
-          for (int b = 0; b < NB; b++)
+        for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) o[b][e] *= f;
-        }
-        v_f = pow2(v_up);
+          for (int e = 0; e < 16; e++) o[b][e] *= f;
       }
-      const bool holes = hole_sh[0] | hole_sh[1] | hole_sh[2] | hole_sh[3];
-      {
-        const float k_f = pow2(k_up);
-        char* to = &k_sh[0][k_row * KS];
-#pragma unroll
-        for (int j = 0; j < KL; j++) {
-          const int at = (4 * j + k_quarter) * PER * 2;
-          if constexpr (TYPE == RTENHIP_CACHE_F16) {
-            *(u32x4*)(to + at) = k_in[j];
-          } else if constexpr (TYPE == RTENHIP_CACHE_BF16) {
-            u32x4 y;
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-              y[e] = __builtin_bit_cast(uint32_t, (f16x2){(_Float16)(cache_lo<TYPE>(k_in[j][e]) * k_f),
-                                                          (_Float16)(cache_hi<TYPE>(k_in[j][e]) * k_f)});
-            *(u32x4*)(to + at) = y;
-          } else {
-            f16x2 h0, l0, h1, l1;
-            split16(__uint_as_float(k_in[j][0]) * k_f, __uint_as_float(k_in[j][1]) * k_f, d.minus1, h0, l0);
-            split16(__uint_as_float(k_in[j][2]) * k_f, __uint_as_float(k_in[j][3]) * k_f, d.minus1, h1, l1);
-            *(f16x4*)(to + at) = (f16x4){h0[0], h0[1], h1[0], h1[1]};
-            *(f16x4*)(to + T::K_BYTES + at) = (f16x4){l0[0], l0[1], l1[0], l1[1]};
-          }
-        }
-        // Keys 4 v_four ..: the 16 they are in, h and i (value_at).
-        const int chunk = (v_four >> 2) * 2 + (v_four & 1), half = (v_four >> 1 & 1) * 8;
-        char* vt = &v_sh[0][half];
-#pragma unroll
-        for (int e = 0; e < DPL; e++) {
-          const int at = value_at(DPL * v_group + e, chunk);
-          if constexpr (TYPE == RTENHIP_CACHE_F16) {
-            const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
-            *(u32x2*)(vt + at) = (u32x2){__builtin_amdgcn_perm(v_in[1][e / 2], v_in[0][e / 2], sel),
-                                         __builtin_amdgcn_perm(v_in[3][e / 2], v_in[2][e / 2], sel)};
-          } else if constexpr (TYPE == RTENHIP_CACHE_BF16) {
-            float x[4];
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-              x[r] = (e & 1 ? cache_hi<TYPE>(v_in[r][e / 2]) : cache_lo<TYPE>(v_in[r][e / 2])) * v_f;
-            *(f16x4*)(vt + at) = (f16x4){(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
-          } else {
-            f16x2 h0, l0, h1, l1;
-            split16(__uint_as_float(v_in[0][e]) * v_f, __uint_as_float(v_in[1][e]) * v_f, d.minus1, h0, l0);
-            split16(__uint_as_float(v_in[2][e]) * v_f, __uint_as_float(v_in[3][e]) * v_f, d.minus1, h1, l1);
-            *(f16x4*)(vt + at) = (f16x4){h0[0], h0[1], h1[0], h1[1]};
-            *(f16x4*)(vt + T::V_BYTES + at) = (f16x4){l0[0], l0[1], l1[0], l1[1]};
-          }
-        }
-        if (k_quarter == 0) seen_sh[k_row] = k_here;
-        if (careful) {
-          if (tid < PA_UNIT) bad_sh[tid] = 0;
-        }
-      }
-      __syncthreads();
-      if (careful) {
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-          if (v_bad[r]) bad_sh[4 * v_four + r] = 1;
-        __syncthreads();
-      }
-      load(u + 1);
-      find_pages(u + 2);
-
-      // Tiles past all of the wave's rows, or before all their windows.
-      const int64_t below_lo = d.window ? (int64_t)pos_lo - d.window : -1;
-      if (!wave_ok || base > pos_hi || (d.window && base + PA_UNIT - 1 <= below_lo && base >= d.sinks)) continue;
-      const int64_t below_hi = d.window ? (int64_t)pos_hi - d.window : -1;
-      const bool whole = !holes && !careful && wave_row + 31 < all_rows && base + PA_UNIT - 1 <= pos_lo &&
-                         base + PA_UNIT <= span.end &&
-                         (base > below_hi || base + PA_UNIT <= d.sinks);
-      const float back = pow2(-q_up - k_up);
-#pragma unroll
-      for (int tb = 0; tb < 2; tb++) {
-        f32x16 s;
-#pragma unroll
-        for (int e = 0; e < 16; e++) s[e] = 0.f;
-        const char* kr = &k_sh[0][(32 * tb + n) * KS + 16 * h];
-#pragma unroll
-        for (int j = 0; j < DP / 16; j++) {
-          const f16x8 a = *(const f16x8*)(kr + 32 * j);
-          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q_hi[j], s, 0, 0, 0);
-          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q_lo[j], s, 0, 0, 0);
-          if constexpr (TERMS == 2) {
-            const f16x8 b = *(const f16x8*)(kr + T::K_BYTES + 32 * j);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, q_hi[j], s, 0, 0, 0);
-          }
-        }
-        if (!whole) {
-#pragma unroll
-          for (int e = 0; e < 16; e += 4) {
-            const int at = base + 32 * tb + 2 * e + 4 * h;
-            const uint32_t here = *(const uint32_t*)&seen_sh[32 * tb + 2 * e + 4 * h];
-            const uint32_t bad = careful ? *(const uint32_t*)&bad_sh[32 * tb + 2 * e + 4 * h] : 0;
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-              const bool seen = (here >> (8 * r) & 1) && at + r <= pos && (at + r > below || at + r < d.sinks);
-              if (!seen) s[e + r] = NEG_INF;
-              poison |= seen && (bad >> (8 * r) & 1);
-            }
-          }
-        }
-        float top = s[0];
-#pragma unroll
-        for (int e = 1; e < 16; e++) top = fmaxf(top, s[e]);
-        top = half_max(top) * back;
-        if (__any(top > m + 6.f)) {
-          const float m_new = fmaxf(m, top);
-          const float fade = __builtin_amdgcn_exp2f(m - (m_new == NEG_INF ? 0.f : m_new));
-          m = m_new;
-          l *= fade;
-#pragma unroll
-          for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) o[b][e] *= fade;
-        }
-        // p 2^8: at most 2^14.
-        const float ref = 8.f - (m == NEG_INF ? 0.f : m);
-        f16x8 p_hi[2], p_lo[2];
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const float a = __builtin_amdgcn_exp2f(__fmaf_rn(s[e], back, ref));
-          const float b = __builtin_amdgcn_exp2f(__fmaf_rn(s[e + 1], back, ref));
-          sum += a + b;
-          f16x2 hi, lo;
-          split16(a, b, d.minus1, hi, lo);
-          p_hi[e >> 3][e & 7] = hi[0], p_hi[e >> 3][(e & 7) + 1] = hi[1];
-          p_lo[e >> 3][e & 7] = lo[0], p_lo[e >> 3][(e & 7) + 1] = lo[1];
-        }
-        l += sum;
-#pragma unroll
-        for (int c = 0; c < 2; c++)
-#pragma unroll
-          for (int b = 0; b < NB; b++) {
-            const int at = value_at(32 * b + n, 2 * (2 * tb + c) + h);
-            const f16x8 a = *(const f16x8*)&v_sh[0][at];
-            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p_hi[c], o[b], 0, 0, 0);
-            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p_lo[c], o[b], 0, 0, 0);
-            if constexpr (TERMS == 2) {
-              const f16x8 z = *(const f16x8*)&v_sh[TERMS - 1][at];
-              o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(z, p_hi[c], o[b], 0, 0, 0);
-            }
-          }
-      }
+      multiply(u, k_exp, some_hole, careful);
+      measure(u + 2, careful);
     }
+    __syncthreads();
   };
   for (int k = 0; k < 2; k++) {
     pass(k);
@@ -1015,11 +1073,11 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void chunk_kernel(Pa
   if (half_max(poison ? 1.f : 0.f) > 0.f) l = __builtin_nanf("");
   if (!row_ok) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const float v_back = SCALED ? pow2(-v_up) : 1.f;
+  const float v_back = SCALED ? pow2(-o_up) : 1.f;
   const int r = wave * 32 + n;
   float* to = w.slot < 0 ? d.out + (int64_t)(w.start + token) * d.o_t + (int64_t)(w.head * d.group + sub) * d.o_h
-                         : d.o_big + ((int64_t)w.slot * PA_BIG + r) * dim;
-  if (w.slot >= 0 && h == 0) d.ml_big[(int64_t)w.slot * PA_BIG + r] = make_float2(m, l);
+                         : d.o_big + ((int64_t)w.slot * T::ROWS + r) * dim;
+  if (w.slot >= 0 && h == 0) d.ml_big[(int64_t)w.slot * T::ROWS + r] = make_float2(m, l);
 #pragma unroll
   for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -1034,40 +1092,69 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void chunk_kernel(Pa
 // ---- merge ---------------------------------------------------------------------------
 
 // out = sum_i l_i 2^(m_i - max m) o_i / sum_i l_i 2^(m_i - max m) over the
-// stretches of a tile.  Workgroup (slot, part) joins its share of the tile's
-// numbers, so a tile of many stretches is joined by as many workgroups.
-template <bool BIG>
+// stretches of a tile.  A tile's numbers are joined 64 at a time, by 16
+// threads for each four of them that take every 16th stretch; the tile's
+// stretches, which are as many slots, divide those 64s among themselves, so a
+// tile of many stretches is joined by many workgroups.
+__device__ __forceinline__ void join(float& m, float& l, f32x4& o, float m2, float l2, const f32x4& o2) {
+  const float top = fmaxf(m, m2), ref = top == NEG_INF ? 0.f : top;
+  const float a = __builtin_amdgcn_exp2f(m - ref), b = __builtin_amdgcn_exp2f(m2 - ref);
+  m = top;
+  l = __fmaf_rn(l, a, l2 * b);
+#pragma unroll
+  for (int e = 0; e < 4; e++) o[e] = __fmaf_rn(o[e], a, o2[e] * b);
+}
+
+constexpr int PA_MERGE_GRID = 512;
+
 __global__ __launch_bounds__(PA_THREADS) void merge_kernel(PagedDesc d) {
-  constexpr int ROWS = BIG ? PA_BIG : PA_SMALL;
-  const Part p = (BIG ? d.part_big : d.part_small)[blockIdx.x];
-  if (p.parts < 2) return;
-  const float* os = BIG ? d.o_big : d.o_small;
-  const float2* ml = BIG ? d.ml_big : d.ml_small;
-  const int slot0 = p.slot - p.part * p.stride;
-  const int dim = d.c.dim, quads = dim / 4, n = p.rows * quads;
-  const int each = (n + p.parts - 1) / p.parts;
-  const int end = min(n, each * (p.part + 1));
-  for (int at = each * p.part + threadIdx.x; at < end; at += PA_THREADS) {
-    const int row = at / quads, c = (at - row * quads) * 4;
-    float m = NEG_INF, l = 0.f;
-    f32x4 sum = {0, 0, 0, 0};
-    for (int i = 0; i < p.parts; i++) {
-      const int64_t slot = slot0 + (int64_t)i * p.stride;
-      const float2 x = ml[slot * ROWS + row];
-      const f32x4 o = *(const f32x4*)(os + (slot * ROWS + row) * dim + c);
-      if (x.y == 0.f) continue;  // saw nothing
-      const float m_new = fmaxf(m, x.x);
-      const float a = __builtin_amdgcn_exp2f(m - m_new), b = __builtin_amdgcn_exp2f(x.x - m_new) * x.y;
-      m = m_new;
-      l = __fmaf_rn(l, a, b);
+  __shared__ float m_sh[4][16], l_sh[4][16];
+  __shared__ f32x4 o_sh[4][16];
+  const int n_small = d.slots_small ? d.slots[0] : 0, n_all = n_small + (d.slots_big ? d.slots[1] : 0);
+  const int tid = threadIdx.x, col = tid & 15, first = tid >> 4, wave = tid >> 6;
+  const int dim = d.c.dim, quads = dim / 4;
+  for (int s = blockIdx.x; s < n_all; s += gridDim.x) {
+    const bool big = s >= n_small;
+    const Part p = big ? d.part_big[s - n_small] : d.part_small[s];
+    const float* os = big ? d.o_big : d.o_small;
+    const float2* ml = big ? d.ml_big : d.ml_small;
+    const int tile_rows = big ? d.rows_big : PA_SMALL;
+    const int slot0 = p.slot - p.part * p.stride;
+    const int n = p.rows * quads;
+    for (int c0 = p.part * 16; c0 < n; c0 += p.parts * 16) {
+      const int at = c0 + col;
+      const int row = min(at, n - 1) / quads, c = (min(at, n - 1) - row * quads) * 4;
+      float m = NEG_INF, l = 0.f;
+      f32x4 o = {0, 0, 0, 0};
+#pragma unroll 4
+      for (int i = first; i < p.parts; i += 16) {
+        const int64_t at_row = (slot0 + (int64_t)i * p.stride) * tile_rows + row;
+        const float2 x = ml[at_row];
+        f32x4 y = *(const f32x4*)(os + at_row * dim + c);
 #pragma unroll
-      for (int e = 0; e < 4; e++) sum[e] = __fmaf_rn(sum[e], a, b * o[e]);
+        for (int e = 0; e < 4; e++) y[e] = x.y == 0.f ? 0.f : y[e] * x.y;
+        join(m, l, o, x.x, x.y, y);
+      }
+#pragma unroll
+      for (int k = 16; k < 64; k <<= 1) {
+        f32x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = __shfl_xor(o[e], k);
+        join(m, l, o, __shfl_xor(m, k), __shfl_xor(l, k), y);
+      }
+      if ((first & 3) == 0) m_sh[wave][col] = m, l_sh[wave][col] = l, o_sh[wave][col] = o;
+      __syncthreads();
+      if (tid < 16 && at < n) {
+#pragma unroll
+        for (int k = 1; k < 4; k++) join(m, l, o, m_sh[k][col], l_sh[k][col], o_sh[k][col]);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] *= inv;
+        const int r = p.row0 + row, token = fdiv(r, d.group_div), sub = r - token * d.group;
+        *(f32x4*)(d.out + (int64_t)(p.token0 + token) * d.o_t + (int64_t)(p.head * d.group + sub) * d.o_h + c) = o;
+      }
+      __syncthreads();
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int r = p.row0 + row, token = fdiv(r, d.group_div), sub = r - token * d.group;
-#pragma unroll
-    for (int e = 0; e < 4; e++) sum[e] *= inv;
-    *(f32x4*)(d.out + (int64_t)(p.token0 + token) * d.o_t + (int64_t)(p.head * d.group + sub) * d.o_h + c) = sum;
   }
 }
 
@@ -1081,7 +1168,7 @@ constexpr int PA_TARGET_SMALL = 1024, PA_TARGET_BIG = 512;
 struct PagedPlan {
   int64_t grid_small, grid_big, slots_small, slots_big;
   size_t bytes;
-  int64_t part_small, part_big, ml_small, ml_big, o_small, o_big;  // offsets in bytes
+  int64_t slots, part_small, part_big, ml_small, ml_big, o_small, o_big;  // offsets in bytes
 };
 
 static rtenhip_status paged_plan(const rtenhip_tensor* q, const rtenhip_kv_cache* cache, const rtenhip_sequences* seqs,
@@ -1104,6 +1191,7 @@ static rtenhip_status paged_plan(const rtenhip_tensor* q, const rtenhip_kv_cache
   d.group = (int)group;
   d.group_div = make_fastdiv((uint32_t)group);
   const int64_t n = seqs->n_seqs, hk = d.c.heads, dim = d.c.dim;
+  d.rows_big = dim <= 64 ? chunk_rows<64>() : dim <= 128 ? chunk_rows<128>() : chunk_rows<256>();
   const int64_t longest = seqs->q_starts ? tokens : std::min<int64_t>(tokens, 1);  // new tokens of a sequence
   const bool small = group <= PA_SMALL, big = longest * group > PA_SMALL;
   // One stretch a tile where no sequence has more than one tile of keys.
@@ -1111,7 +1199,7 @@ static rtenhip_status paged_plan(const rtenhip_tensor* q, const rtenhip_kv_cache
   p = PagedPlan{};
   if (tokens && n) {
     const int64_t small_tiles = std::min(n, tokens) * hk;
-    const int64_t big_tiles = (tokens * group / PA_BIG + std::min(n, tokens)) * hk;
+    const int64_t big_tiles = (tokens * group / d.rows_big + std::min(n, tokens)) * hk;
     if (small) p.grid_small = small_tiles + (splits ? PA_TARGET_SMALL : 0);
     if (big) p.grid_big = big_tiles + (splits ? PA_TARGET_BIG : 0);
     if (p.grid_small > INT32_MAX || p.grid_big > INT32_MAX)
@@ -1128,12 +1216,13 @@ static rtenhip_status paged_plan(const rtenhip_tensor* q, const rtenhip_kv_cache
     return (int64_t)here;
   };
   if (splits) {
-    p.part_small = take(p.grid_small * (int64_t)sizeof(Part));
-    p.part_big = take(p.grid_big * (int64_t)sizeof(Part));
+    p.slots = take(2 * (int64_t)sizeof(int));
+    p.part_small = take(p.slots_small * (int64_t)sizeof(Part));
+    p.part_big = take(p.slots_big * (int64_t)sizeof(Part));
     p.ml_small = take(p.slots_small * PA_SMALL * (int64_t)sizeof(float2));
-    p.ml_big = take(p.slots_big * PA_BIG * (int64_t)sizeof(float2));
+    p.ml_big = take(p.slots_big * d.rows_big * (int64_t)sizeof(float2));
     p.o_small = take(p.slots_small * PA_SMALL * dim * 4);
-    p.o_big = take(p.slots_big * PA_BIG * dim * 4);
+    p.o_big = take(p.slots_big * d.rows_big * dim * 4);
   }
   p.bytes = at;
   return RTENHIP_OK;
@@ -1144,7 +1233,7 @@ static void launch_paged(const PagedDesc& d, hipStream_t s) {
   if (d.grid_small)
     hipLaunchKernelGGL((decode_kernel<DP, TYPE>), dim3((unsigned)d.grid_small), dim3(PA_THREADS), 0, s, d);
   if (d.grid_big)
-    hipLaunchKernelGGL((chunk_kernel<DP, TYPE>), dim3((unsigned)d.grid_big), dim3(PA_THREADS), 0, s, d);
+    hipLaunchKernelGGL((chunk_kernel<DP, TYPE>), dim3((unsigned)d.grid_big), dim3(ChunkTile<DP, TYPE>::THREADS), 0, s, d);
 }
 
 template <int TYPE>
@@ -1202,6 +1291,7 @@ extern "C" rtenhip_status rtenhip_paged_attention_f32(rtenhip_ctx* ctx, const rt
   d.target_small = PA_TARGET_SMALL, d.target_big = PA_TARGET_BIG;
   char* ws = (char*)workspace;
   if (p.bytes) {
+    d.slots = (int*)(ws + p.slots);
     d.part_small = (Part*)(ws + p.part_small);
     d.part_big = (Part*)(ws + p.part_big);
     d.ml_small = (float2*)(ws + p.ml_small);
@@ -1216,8 +1306,9 @@ extern "C" rtenhip_status rtenhip_paged_attention_f32(rtenhip_ctx* ctx, const rt
   else if (dtype == RTENHIP_CACHE_F16) launch_paged<RTENHIP_CACHE_F16>(d, s);
   else launch_paged<RTENHIP_CACHE_BF16>(d, s);
   RTENHIP_LAUNCH_CHECK();
-  if (p.slots_small) hipLaunchKernelGGL((merge_kernel<false>), dim3((unsigned)p.grid_small), dim3(PA_THREADS), 0, s, d);
-  if (p.slots_big) hipLaunchKernelGGL((merge_kernel<true>), dim3((unsigned)p.grid_big), dim3(PA_THREADS), 0, s, d);
-  RTENHIP_LAUNCH_CHECK();
+  if (p.slots_small || p.slots_big) {
+    hipLaunchKernelGGL(merge_kernel, dim3(PA_MERGE_GRID), dim3(PA_THREADS), 0, s, d);
+    RTENHIP_LAUNCH_CHECK();
+  }
   return RTENHIP_OK;
 }

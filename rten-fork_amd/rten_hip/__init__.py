@@ -190,8 +190,8 @@ class Context:
     def sync_stream(self, stream=None):
         torch = _torch()
         s = stream if stream is not None else torch.cuda.current_stream(self.device)
-        self.stream = s
-        check(lib().rtenhip_set_stream(C.c_void_p(self.ptr), C.c_void_p(s.cuda_stream)))
+        check(lib().rtenhip_set_stream(self.ptr, s.cuda_stream))
+        self.stream = s  # the torch stream the context's work is queued on
 
     def use_stream(self, stream):
         """Run this context's graphs on ``stream`` (a torch.cuda.Stream) and

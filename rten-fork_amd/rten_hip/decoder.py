@@ -17,10 +17,9 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 
-from . import OpError, Tensor, _torch, check, default_context, lib
-
-CACHE_DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+from . import OpError, Tensor, _torch, check, default_context, lib  # noqa: F401  (Tensor: the row descriptors' layout)
 
 
 class KVCache(C.Structure):
@@ -61,6 +60,16 @@ _SIGNATURES = {
 }
 _functions = {}
 
+# A call's descriptors as bytes in the structures' layouts: packing one takes
+# a third of filling a ctypes structure, and a step of a decoder makes hundreds
+# of calls that the GPU is done with in a few microseconds each.
+_ROWS = struct.Struct("Pi4x3q40x3q40x")
+_MATRIX = struct.Struct("Pi4x2q48x2q48x")
+_CACHE = struct.Struct("PPiiqii3q3q")
+_SEQUENCES = struct.Struct("PqPPii")
+_ROTARY = struct.Struct("PPPPfii4x")
+_SAMPLING = struct.Struct("fffiPPPP")
+
 
 def _call(name, *args):
     f = _functions.get(name)
@@ -68,7 +77,9 @@ def _call(name, *args):
         f = getattr(lib(), name)
         f.argtypes, f.restype = _SIGNATURES[name], C.c_int
         _functions[name] = f
-    check(f(*args))
+    code = f(*args)
+    if code:
+        check(code)
 
 
 def _on_device(t, ctx, dtype, what):
@@ -79,19 +90,19 @@ def _on_device(t, ctx, dtype, what):
 
 
 def _rows(t, ctx, what):
-    """rtenhip_tensor of a float32 [tokens, heads, head_dim] (or [rows, vocab]) tensor."""
+    """rtenhip_tensor of a float32 [tokens, heads, head_dim] tensor."""
     _on_device(t, ctx, _torch().float32, what)
-    if t.dim() > 8:
-        raise OpError(6, "too many dims")
-    return Tensor(t.data_ptr() if t.numel() else None, t.dim(), tuple(t.shape), tuple(t.stride()))
+    if t.dim() != 3:
+        raise OpError(3, "Expected [tokens, heads, head_dim] inputs")
+    return _ROWS.pack(t.data_ptr(), 3, *t.shape, *t.stride())
 
 
 def _vector(t, n, ctx, dtype, what):
     """Address of a contiguous 1-D device tensor of n elements (None: NULL)."""
     if t is None:
-        return None
+        return 0
     _on_device(t, ctx, dtype, what)
-    if t.dim() != 1 or t.shape[0] != n:
+    if t.shape != (n,):
         raise OpError(3, f"{what} must have {n} elements")
     if n > 1 and t.stride(0) != 1:
         raise OpError(6, f"{what} must be contiguous")
@@ -99,54 +110,87 @@ def _vector(t, n, ctx, dtype, what):
 
 
 def _cache(k, v, ctx):
-    if k.dim() != 4 or k.shape != v.shape:
+    """rtenhip_kv_cache of two [pages, page size, heads, head_dim] tensors."""
+    shape, dtype = k.shape, k.dtype
+    if len(shape) != 4 or v.shape != shape:
         raise OpError(3, "Caches must be [pages, page size, heads, head_dim] of the same shape")
-    if str(k.dtype) not in CACHE_DTYPES:
-        raise OpError(1, "IncorrectInputType: cache must be float32, float16 or bfloat16")
-    _on_device(k, ctx, k.dtype, "cache")
-    _on_device(v, ctx, k.dtype, "cache")
-    n, page, heads, dim = k.shape
-    ks, vs = k.stride(), v.stride()
-    if dim > 1 and (ks[3] != 1 or vs[3] != 1):
+    kind = _cache_dtype(dtype)
+    _on_device(k, ctx, dtype, "cache")
+    _on_device(v, ctx, dtype, "cache")
+    n, page, heads, dim = shape
+    k0, k1, k2, k3 = k.stride()
+    v0, v1, v2, v3 = v.stride()
+    if dim > 1 and (k3 != 1 or v3 != 1):
         raise OpError(6, "Cache rows must have unit stride")
-    if page > 65536:
+    if max(page, heads, dim) > 0x7fffffff:
         raise OpError(5, "Invalid cache size")
-    return KVCache(k.data_ptr() if n else None, v.data_ptr() if n else None, CACHE_DTYPES[str(k.dtype)], page, n, heads,
-                   dim, ks[:3], vs[:3])
+    return _CACHE.pack(k.data_ptr(), v.data_ptr(), kind, page, n, heads, dim, k0, k1, k2, v0, v1, v2)
+
+
+_cache_dtypes = {}
+
+
+def _cache_dtype(dtype):
+    if not _cache_dtypes:
+        torch = _torch()
+        _cache_dtypes.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+    kind = _cache_dtypes.get(dtype)
+    if kind is None:
+        raise OpError(1, "IncorrectInputType: cache must be float32, float16 or bfloat16")
+    return kind
 
 
 def _sequences(page_table, kv_lens, q_starts, ctx):
+    """rtenhip_sequences."""
     i32 = _torch().int32
     _on_device(page_table, ctx, i32, "page_table")
     if page_table.dim() != 2:
         raise OpError(3, "page_table must be [sequences, pages]")
     n, pages = page_table.shape
-    if pages > 1 and page_table.stride(1) != 1:
+    row, unit = page_table.stride()
+    if pages > 1 and unit != 1:
         raise OpError(6, "page_table rows must have unit stride")
-    return Sequences(page_table.data_ptr() if n * pages else None, page_table.stride(0),
-                     _vector(kv_lens, n, ctx, i32, "kv_lens"), _vector(q_starts, n + 1, ctx, i32, "q_starts"), n, pages)
+    return _SEQUENCES.pack(page_table.data_ptr(), row, _vector(kv_lens, n, ctx, i32, "kv_lens"),
+                           _vector(q_starts, n + 1, ctx, i32, "q_starts"), n, pages)
 
 
-def _empty(shape, dtype, ctx):
-    """A tensor whose memory belongs to the context's stream, which is the one
-    that the call writes it on."""
+def _context(ctx):
+    """The context of a call and whether torch allocates on its stream: the
+    default context follows torch's current stream."""
+    if ctx is None:
+        return default_context(), True
     torch = _torch()
-    device = torch.device("cuda", ctx.device)
-    if ctx.stream.cuda_stream == torch.cuda.current_stream(ctx.device).cuda_stream:
-        return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(ctx.stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+    return ctx, ctx.stream.cuda_stream == torch.cuda.current_stream(ctx.device).cuda_stream
+
+
+def _empty(like, shape, dtype, ctx, here):
+    """A tensor on like's device whose memory belongs to the context's stream,
+    which is the one that the call writes it on."""
+    if here:
+        return like.new_empty(shape, dtype=dtype)
+    with _torch().cuda.stream(ctx.stream):
+        return like.new_empty(shape, dtype=dtype)
 
 
 def _rotary(inv_freq, positions, tokens, dim, q_scale, k_scale, epsilon, interleaved, ctx):
+    """rtenhip_rotary."""
     torch = _torch()
     f32 = torch.float32
-    half = 0 if inv_freq is None else inv_freq.shape[0] if inv_freq.dim() == 1 else -1
-    if half < 0:
-        raise OpError(3, "inv_freq must be 1-D")
-    return Rotary(_vector(q_scale, dim, ctx, f32, "q_scale"), _vector(k_scale, dim, ctx, f32, "k_scale"),
-                  _vector(inv_freq, half, ctx, f32, "inv_freq"),
-                  _vector(positions, tokens, ctx, torch.int32, "positions"), epsilon, 2 * half, int(bool(interleaved)))
+    half = 0
+    if inv_freq is not None:
+        if inv_freq.dim() != 1:
+            raise OpError(3, "inv_freq must be 1-D")
+        half = inv_freq.shape[0]
+        if half > 128:
+            raise OpError(6, "rotary_dim must be a multiple of 8 up to head_dim")
+    return _ROTARY.pack(_vector(q_scale, dim, ctx, f32, "q_scale"), _vector(k_scale, dim, ctx, f32, "k_scale"),
+                        _vector(inv_freq, half, ctx, f32, "inv_freq"),
+                        _vector(positions, tokens, ctx, torch.int32, "positions"), epsilon, 2 * half,
+                        1 if interleaved else 0)
+
+
+def _int32(n):
+    return max(-1, min(int(n), 0x7fffffff))
 
 
 def _check_3d(*tensors):
@@ -163,15 +207,15 @@ def qk_norm_rotary(q, k, positions, inv_freq, q_scale=None, k_scale=None, epsilo
     ``inv_freq`` has rotary_dim / 2 values (None: no rotation); pairs are
     (i, i + rotary_dim / 2), or neighbours if ``interleaved``.  Returns
     (q_out, k_out); either may be given, its input itself included."""
-    ctx = ctx or default_context()
+    ctx, here = _context(ctx)
     _check_3d(q, k)
     r = _rotary(inv_freq, positions, q.shape[0], q.shape[2], q_scale, k_scale, epsilon, interleaved, ctx)
     if q_out is None:
-        q_out = _empty(q.shape, q.dtype, ctx)
+        q_out = _empty(q, q.shape, q.dtype, ctx, here)
     if k_out is None:
-        k_out = _empty(k.shape, k.dtype, ctx)
-    qd, kd, qo, ko = _rows(q, ctx, "q"), _rows(k, ctx, "k"), _rows(q_out, ctx, "q_out"), _rows(k_out, ctx, "k_out")
-    _call("rtenhip_qk_norm_rotary_f32", ctx.ptr, C.byref(qd), C.byref(kd), C.byref(r), C.byref(qo), C.byref(ko))
+        k_out = _empty(k, k.shape, k.dtype, ctx, here)
+    _call("rtenhip_qk_norm_rotary_f32", ctx.ptr, _rows(q, ctx, "q"), _rows(k, ctx, "k"), r, _rows(q_out, ctx, "q_out"),
+          _rows(k_out, ctx, "k_out"))
     return q_out, k_out
 
 
@@ -181,16 +225,15 @@ def qk_norm_rotary_append(q, k, v, inv_freq, k_cache, v_cache, page_table, kv_le
     and v written into the cache.  ``positions`` (default: the tokens' places
     in their sequences) turn the rows only.  Returns q's rows (``out``, which
     may be q); rows of padding in a new ``out`` are not initialised."""
-    ctx = ctx or default_context()
+    ctx, here = _context(ctx)
     _check_3d(q, k, v)
     r = _rotary(inv_freq, positions, q.shape[0], q.shape[2], q_scale, k_scale, epsilon, interleaved, ctx)
     cache = _cache(k_cache, v_cache, ctx)
     seqs = _sequences(page_table, kv_lens, q_starts, ctx)
     if out is None:
-        out = _empty(q.shape, q.dtype, ctx)
-    qd, kd, vd, od = _rows(q, ctx, "q"), _rows(k, ctx, "k"), _rows(v, ctx, "v"), _rows(out, ctx, "out")
-    _call("rtenhip_qk_norm_rotary_append_f32", ctx.ptr, C.byref(qd), C.byref(kd), C.byref(vd), C.byref(r),
-          C.byref(cache), C.byref(seqs), C.byref(od))
+        out = _empty(q, q.shape, q.dtype, ctx, here)
+    _call("rtenhip_qk_norm_rotary_append_f32", ctx.ptr, _rows(q, ctx, "q"), _rows(k, ctx, "k"), _rows(v, ctx, "v"), r,
+          cache, seqs, _rows(out, ctx, "out"))
     return out
 
 
@@ -202,20 +245,18 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_lens, q_starts=None, sca
     up to p; with a ``window``, the last ``window`` of them and the first
     ``sinks``.  ``scale`` defaults to 1 / sqrt(head_dim).  A row that sees
     nothing gives zeros; rows of padding in a new ``out`` are not initialised."""
-    ctx = ctx or default_context()
+    ctx, here = _context(ctx)
     cache = _cache(k_cache, v_cache, ctx)
     seqs = _sequences(page_table, kv_lens, q_starts, ctx)
     qd = _rows(q, ctx, "q")
     if out is None:
-        out = _empty(q.shape, q.dtype, ctx)
-    od = _rows(out, ctx, "out")
+        out = _empty(q, q.shape, q.dtype, ctx, here)
     need = C.c_size_t()
-    _call("rtenhip_paged_attention_workspace", C.byref(qd), C.byref(cache), C.byref(seqs), C.byref(need))
+    _call("rtenhip_paged_attention_workspace", qd, cache, seqs, C.byref(need))
     n = need.value
-    ws = _empty((n,), _torch().uint8, ctx) if n else None
-    _call("rtenhip_paged_attention_f32", ctx.ptr, C.byref(qd), C.byref(cache), C.byref(seqs),
-          1 / math.sqrt(cache.head_dim) if scale is None else scale, window, sinks, ws.data_ptr() if n else None, n,
-          C.byref(od))
+    ws = _empty(q, (n,), _torch().uint8, ctx, here) if n else None
+    _call("rtenhip_paged_attention_f32", ctx.ptr, qd, cache, seqs, 1 / math.sqrt(q.shape[2]) if scale is None else scale,
+          _int32(window), _int32(sinks), ws.data_ptr() if n else None, n, _rows(out, ctx, "out"))
     return out
 
 
@@ -226,25 +267,25 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ctx
     ``top_p`` 1 and ``min_p`` 0 keep all, ``temperature`` 0 takes the largest)
     are numbers, or device tensors with one for each row."""
     torch = _torch()
-    ctx = ctx or default_context()
-    ld = _rows(logits, ctx, "logits")
+    ctx, here = _context(ctx)
+    f32, i32 = torch.float32, torch.int32
+    _on_device(logits, ctx, f32, "logits")
     if logits.dim() != 2:
         raise OpError(3, "Expected [rows, vocab] logits")
     rows, vocab = logits.shape
-    s = Sampling(1.0, 1.0, 0.0, 0)
-    for name, value in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p), ("top_k", top_k)):
-        if isinstance(value, torch.Tensor):
-            dtype = torch.int32 if name == "top_k" else torch.float32
-            setattr(s, name + "s", _vector(value, rows, ctx, dtype, name))
-        elif name == "top_k":
-            s.top_k = min(max(int(value), 0), vocab)
-        else:
-            setattr(s, name, value)
-    u = _vector(uniforms, rows, ctx, torch.float32, "uniforms")
-    tokens, logprobs = _empty((rows,), torch.int32, ctx), _empty((rows,), torch.float32, ctx)
+
+    def per_row(value, dtype, what):
+        return _vector(value, rows, ctx, dtype, what) if isinstance(value, torch.Tensor) else 0
+
+    t, k = per_row(temperature, f32, "temperature"), per_row(top_k, i32, "top_k")
+    p, m = per_row(top_p, f32, "top_p"), per_row(min_p, f32, "min_p")
+    s = _SAMPLING.pack(1. if t else temperature, 1. if p else top_p, 0. if m else min_p,
+                       0 if k else min(max(int(top_k), 0), vocab), t, p, m, k)
+    u = _vector(uniforms, rows, ctx, f32, "uniforms")
     need = C.c_size_t()
     _call("rtenhip_sample_workspace", rows, vocab, C.byref(need))
-    ws = _empty((need.value,), torch.uint8, ctx)
-    _call("rtenhip_sample_f32", ctx.ptr, C.byref(ld), C.byref(s), u, ws.data_ptr(), need.value, tokens.data_ptr(),
-          logprobs.data_ptr())
+    tokens, logprobs = _empty(logits, (rows,), i32, ctx, here), _empty(logits, (rows,), f32, ctx, here)
+    ws = _empty(logits, (need.value,), torch.uint8, ctx, here)
+    _call("rtenhip_sample_f32", ctx.ptr, _MATRIX.pack(logits.data_ptr(), 2, rows, vocab, *logits.stride()), s, u,
+          ws.data_ptr(), need.value, tokens.data_ptr(), logprobs.data_ptr())
     return tokens, logprobs

@@ -277,3 +277,25 @@ def test_python_binding_refuses_before_the_library(d):
                       (c, c, "GPU")):
         with pytest.raises(OpError, match=msg):
             d._cache(k, v, Ctx)
+
+
+def test_packed_descriptors_have_the_structures_layouts(d):
+    """The bytes that the binding passes, field by field."""
+    def same(kind, packed, **fields):
+        s = kind.from_buffer_copy(packed)
+        assert C.sizeof(kind) == len(packed)
+        for name, want in fields.items():
+            got = getattr(s, name)
+            assert (tuple(got) if hasattr(got, "__len__") else got) == want, name
+
+    same(d.Tensor, d._ROWS.pack(7, 3, 1, 2, 3, 6, 5, 4), data=7, ndim=3, shape=(1, 2, 3, 0, 0, 0, 0, 0),
+         strides=(6, 5, 4, 0, 0, 0, 0, 0))
+    same(d.Tensor, d._MATRIX.pack(7, 2, 1, 2, 6, 5), data=7, ndim=2, shape=(1, 2) + (0,) * 6, strides=(6, 5) + (0,) * 6)
+    same(d.KVCache, d._CACHE.pack(1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13), k=1, v=2, dtype=3, page_size=4, n_pages=5,
+         n_heads=6, head_dim=7, k_strides=(8, 9, 10), v_strides=(11, 12, 13))
+    same(d.Sequences, d._SEQUENCES.pack(1, 2, 3, 4, 5, 6), page_table=1, table_stride=2, kv_lens=3, q_starts=4, n_seqs=5,
+         max_pages=6)
+    same(d.Rotary, d._ROTARY.pack(1, 2, 3, 4, 0.5, 6, 7), q_scale=1, k_scale=2, inv_freq=3, positions=4, epsilon=0.5,
+         rotary_dim=6, interleaved=7)
+    same(d.Sampling, d._SAMPLING.pack(0.5, 0.25, 0.125, 4, 5, 6, 7, 8), temperature=0.5, top_p=0.25, min_p=0.125, top_k=4,
+         temperatures=5, top_ps=6, min_ps=7, top_ks=8)
