@@ -99,6 +99,11 @@ __device__ __forceinline__ Span span_of(const PagedDesc& d, int kv_len, int p0, 
   return v;
 }
 
+// The last key that position `pos` sees as a sink only, -1 without a window.
+__device__ __forceinline__ int sinks_only(const PagedDesc& d, int pos) {
+  return d.window ? max(-1, (int)max((int64_t)pos - d.window, (int64_t)-1)) : -1;
+}
+
 struct Work {
   int seq, start, q_len, kv_len;
   int tile, head, part, parts, slot;
@@ -209,7 +214,13 @@ __device__ bool plan(const PagedDesc& d, int block, PlanShared& sh, Work& out) {
     }
   }
   __syncthreads();
-  out = sh.work;
+  // (In scalar registers: everything that follows from it is the same for all
+  // lanes, loops and addresses among it.)
+  static_assert(sizeof(Work) % 4 == 0, "copied word by word");
+  const int* from = (const int*)&sh.work;
+  int* to = (int*)&out;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(Work) / 4); i++) to[i] = __builtin_amdgcn_readfirstlane(from[i]);
   return out.seq >= 0;
 }
 
@@ -295,31 +306,38 @@ struct DecodeTile {
   static constexpr int QW = TYPE == RTENHIP_CACHE_F32 ? DP / 4 : TYPE == RTENHIP_CACHE_F16 ? DP / 4 : 3 * DP / 8;
 };
 
+// (Past head_dim the row's last 16 bytes again: q is zero there, and those
+// results are not stored.)
 template <int DP, int TYPE>
-__device__ __forceinline__ void load_keys(const char* row, bool ok, int g, int dim, u32x4* k) {
+__device__ __forceinline__ void load_keys(const char* base, int64_t row, int g, int dim, u32x4* k) {
   constexpr int KV = DecodeTile<DP, TYPE>::KV, size = CacheType<TYPE>::size, per = 16 / size;
 #pragma unroll
-  for (int j = 0; j < KV; j++) {
-    const int at = (4 * j + g) * per;
-    k[j] = (u32x4){0, 0, 0, 0};
-    if (ok && at < dim) k[j] = *(const u32x4*)(row + at * size);
+  for (int j = 0; j < KV; j++) k[j] = (u32x4){0, 0, 0, 0};
+  if (row >= 0) {
+#pragma unroll
+    for (int j = 0; j < KV; j++) k[j] = *(const u32x4*)(base + row + min((4 * j + g) * per, dim - per) * size);
   }
 }
 
-template <int DP, int TYPE>
-__device__ __forceinline__ void load_values(const char* row, bool ok, int i, int dim, uint32_t* v) {
-  constexpr int VW = DecodeTile<DP, TYPE>::VW, DPL = DP / 16, size = CacheType<TYPE>::size;
-  if constexpr (VW == 2) {
-    u32x2 x = {0, 0};
-    if (ok && i * DPL < dim) x = *(const u32x2*)(row + i * DPL * size);
+// WORDS words at byte `at` of a row of `bytes` (zero if row < 0), the row's
+// last ones where there are fewer.
+template <int WORDS>
+__device__ __forceinline__ void load_words(const char* base, int64_t row, int at, int bytes, uint32_t* v) {
+#pragma unroll
+  for (int c = 0; c < WORDS; c++) v[c] = 0;
+  if (row < 0) return;
+  const char* p = base + row;
+  if constexpr (WORDS == 1) {
+    v[0] = *(const uint32_t*)(p + min(at, bytes - 4));
+  } else if constexpr (WORDS == 2) {
+    const u32x2 x = *(const u32x2*)(p + min(at, bytes - 8));
     v[0] = x[0], v[1] = x[1];
   } else {
 #pragma unroll
-    for (int c = 0; c < VW / 4; c++) {
-      u32x4 x = {0, 0, 0, 0};
-      if (ok && i * DPL + c * (16 / size) < dim) x = *(const u32x4*)(row + i * DPL * size + c * 16);
+    for (int c = 0; c < WORDS; c += 4) {
+      const u32x4 x = *(const u32x4*)(p + min(at + 4 * c, bytes - 16));
 #pragma unroll
-      for (int e = 0; e < 4; e++) v[4 * c + e] = x[e];
+      for (int e = 0; e < 4; e++) v[c + e] = x[e];
     }
   }
 }
@@ -352,13 +370,13 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
   if (!plan<false, PA_THREADS, PA_SMALL>(d, blockIdx.x, plan_sh, w) || w.slot >= d.slots_small) return;
   if (threadIdx.x == 0 && w.slot >= 0)
     d.part_small[w.slot] = Part{w.slot, w.part, w.parts, d.c.heads, w.start, 0, w.q_len * d.group, w.head};
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int i = lane & 15, g = lane >> 4;
   const int dim = d.c.dim, rows = w.q_len * d.group;
   const int token = fdiv(i, d.group_div), sub = i - token * d.group;
   const bool row_ok = i < rows;
   const int pos = row_ok ? w.kv_len - w.q_len + token : -1;
-  const int64_t below = d.window ? (int64_t)pos - d.window : -1;  // keys up to here are seen as sinks only
+  const int below = sinks_only(d, pos);
 
   // Q, times scale log2 e, as the matrix instructions take it.
   uint32_t qw[T::QW];
@@ -424,16 +442,20 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
   const char* kc = d.c.k + (int64_t)w.head * d.c.k_head * size;
   const char* vc = d.c.v + (int64_t)w.head * d.c.v_head * size;
 
-  // The page of the lane's key (key i of the wave's 16) in tile u, -1 where no
-  // row sees the key.
-  auto page_at = [&](int u, int& key) {
-    key = 0;
+  // The lane's key (key i of the wave's 16) in tile u: its page, and its rows'
+  // offsets from that, -1 where no row sees the key or it has no page.
+  auto page_at = [&](int u) {
     if (u >= u1) return -1;
-    key = span.tile(u) * PA_UNIT + 16 * wave + i;
+    const int key = span.tile(u) * PA_UNIT + 16 * wave + i;
     if (key >= span.end || (key < span.lo && key >= d.sinks)) return -1;
     return page_of(table, d.s.max_pages, d.c, key);
   };
-  auto slot_of = [&](int key) { return key - fdiv(key, d.c.page_div) * d.c.page_size; };
+  auto rows_at = [&](int u, int page, int64_t& k_row, int64_t& v_row) {
+    const int key = (u < u1 ? span.tile(u) * PA_UNIT : 0) + 16 * wave + i;
+    const int64_t slot = key - fdiv(key, d.c.page_div) * d.c.page_size;
+    k_row = page < 0 ? -1 : (page * d.c.k_page + slot * d.c.k_slot) * size;
+    v_row = page < 0 ? -1 : (page * d.c.v_page + slot * d.c.v_slot) * size;
+  };
 
   float m, l;
   f32x4 o[DPL];
@@ -443,27 +465,26 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
     poison = false;
 #pragma unroll
     for (int e = 0; e < DPL; e++) o[e] = (f32x4){0, 0, 0, 0};
-    int key, key_next;
-    int page = page_at(u0, key), page_next = page_at(u0 + 1, key_next);
+    int page_next = page_at(u0);
+    int64_t k_row, v_row;
+    rows_at(u0, page_next, k_row, v_row);
+    page_next = page_at(u0 + 1);
     u32x4 k[KV], k_next[KV];
-    load_keys<DP, TYPE>(kc + ((int64_t)page * d.c.k_page + (int64_t)slot_of(key) * d.c.k_slot) * size, page >= 0, g,
-                        dim, k);
+    load_keys<DP, TYPE>(kc, k_row, g, dim, k);
     for (int u = u0; u < u1; u++) {
       // This tile's values, the next one's keys, the one after's pages.
-      int vpage[4];
+      bool here[4];
       uint32_t v[4][VW];
       const int base = span.tile(u) * PA_UNIT + 16 * wave + 4 * g;
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        vpage[r] = __shfl(page, 4 * g + r);
-        load_values<DP, TYPE>(vc + ((int64_t)vpage[r] * d.c.v_page + (int64_t)slot_of(base + r) * d.c.v_slot) * size,
-                              vpage[r] >= 0, i, dim, v[r]);
+        const int64_t row = __shfl((long long)v_row, 4 * g + r);
+        here[r] = row >= 0;
+        load_words<VW>(vc, row, i * DPL * size, dim * size, v[r]);
       }
-      load_keys<DP, TYPE>(
-          kc + ((int64_t)page_next * d.c.k_page + (int64_t)slot_of(key_next) * d.c.k_slot) * size, page_next >= 0, g,
-          dim, k_next);
-      page = page_next;
-      page_next = page_at(u + 2, key_next);
+      rows_at(u + 1, page_next, k_row, v_row);
+      load_keys<DP, TYPE>(kc, k_row, g, dim, k_next);
+      page_next = page_at(u + 2);
 
       f32x4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
 #pragma unroll
@@ -499,7 +520,7 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         const int at = base + r;
-        seen[r] = vpage[r] >= 0 && at <= pos && (at > below || at < d.sinks);
+        seen[r] = here[r] && at <= pos && (at > below || at < d.sinks);
         p[r] = seen[r] ? (s0[r] + s1[r]) * q_back : NEG_INF;
         top = fmaxf(top, p[r]);
       }
@@ -684,6 +705,13 @@ __device__ __forceinline__ int value_at(int dimension, int chunk) {
   if constexpr (TN == 64) return dimension * 128 + ((chunk ^ dimension ^ (dimension >> 3)) & 7) * 16;
   return dimension * 64 + ((chunk ^ (dimension >> 1) ^ (dimension >> 3)) & 3) * 16;
 }
+// value_at(32 b + n, chunk + h) for n < 32, even chunks and h < 2 is
+// value_at(n, h) with these bits flipped and 32 b rows on.
+template <int TN>
+__device__ __forceinline__ constexpr int value_flip(int dimension, int chunk) {
+  if (TN == 64) return ((chunk ^ (dimension >> 3)) & 7) * 16;
+  return ((chunk ^ (dimension >> 1) ^ (dimension >> 3)) & 3) * 16;
+}
 
 template <int TYPE>
 __device__ __forceinline__ float cache_lo(uint32_t w) {
@@ -703,26 +731,6 @@ __device__ __forceinline__ float top_of(float top, uint32_t w) {
   return fmaxf(top, fmaxf(fabsf(cache_lo<TYPE>(w)), fabsf(cache_hi<TYPE>(w))));
 }
 
-template <int WORDS>
-__device__ __forceinline__ void load_words(const char* p, bool ok, uint32_t* v) {
-#pragma unroll
-  for (int c = 0; c < WORDS; c++) v[c] = 0;
-  if (!ok) return;
-  if constexpr (WORDS == 1) {
-    v[0] = *(const uint32_t*)p;
-  } else if constexpr (WORDS == 2) {
-    const u32x2 x = *(const u32x2*)p;
-    v[0] = x[0], v[1] = x[1];
-  } else {
-#pragma unroll
-    for (int c = 0; c < WORDS; c += 4) {
-      const u32x4 x = *(const u32x4*)(p + 4 * c);
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[c + e] = x[e];
-    }
-  }
-}
-
 template <int DP, int TYPE>
 __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) void chunk_kernel(PagedDesc d) {
   using T = ChunkTile<DP, TYPE>;
@@ -732,8 +740,12 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
   __shared__ PlanShared plan_sh;
   __shared__ __attribute__((aligned(16))) char buffer_sh[2][T::BUFFER];  // keys hi, lo, values hi, lo
   __shared__ float top_sh[2][2][WAVES];                                  // [tile & 1][keys, values]
-  __shared__ int hole_sh[2][WAVES];
-  __shared__ __attribute__((aligned(4))) uint8_t seen_sh[4][TN], bad_sh[4][TN];  // [tile & 3]: read late
+  // [tile & 3], as they are read late: the keys' rows [keys, values], those
+  // that somebody sees, whether one lacks its page, whose value is not finite.
+  __shared__ int64_t rows_sh[4][2][TN];
+  __shared__ uint64_t seen_sh[4];
+  __shared__ int hole_sh[4];
+  __shared__ __attribute__((aligned(4))) uint8_t bad_sh[4][TN];
   Work w;
   if (!plan<true, T::THREADS, T::ROWS>(d, blockIdx.x, plan_sh, w) || w.slot >= d.slots_big) return;
   const int row0 = w.tile * T::ROWS;
@@ -741,7 +753,7 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
   const int rows = min(T::ROWS, all_rows - row0);
   if (threadIdx.x == 0 && w.slot >= 0)
     d.part_big[w.slot] = Part{w.slot, w.part, w.parts, d.c.heads, w.start, row0, rows, w.head};
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int n = lane & 31, h = lane >> 5;
   const int dim = d.c.dim, first = w.kv_len - w.q_len;
   const int wave_row = row0 + wave * 32;
@@ -750,10 +762,11 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
   const bool row_ok = row < all_rows;
   const int token = fdiv(row_ok ? row : 0, d.group_div), sub = row_ok ? row - token * d.group : 0;
   const int pos = row_ok ? first + token : -1;
-  const int64_t below = d.window ? (int64_t)pos - d.window : -1;
+  const int below = sinks_only(d, pos);
   // The first and the last position of the wave's rows.
   const int pos_lo = wave_ok ? first + fdiv(wave_row, d.group_div) : 0;
   const int pos_hi = wave_ok ? first + fdiv(min(wave_row + 31, all_rows - 1), d.group_div) : -1;
+  const int below_lo = sinks_only(d, pos_lo), below_hi = sinks_only(d, pos_hi);
 
   f16x8 q_hi[DP / 16], q_lo[DP / 16];
   int q_up;
@@ -786,6 +799,7 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
       }
   }
 
+  const int v_base = value_at<TN>(n, h);
   const Span span = span_of<TN>(d, w.kv_len, first + fdiv(row0, d.group_div),
                                 first + fdiv(row0 + rows - 1, d.group_div));
   const int u0 = (int)((int64_t)span.tiles * w.part / w.parts), u1 = (int)((int64_t)span.tiles * (w.part + 1) / w.parts);
@@ -798,39 +812,47 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
   const int k_row = tid >> 3, k_eighth = tid & 7, v_group = tid & 31;
   const int v_chunk = (tid >> 7) * 2 + (tid >> 6 & 1), v_half = tid >> 5 & 1;
   const int v_key = 16 * (tid >> 7) + 8 * v_half + 4 * (tid >> 6 & 1);
-  auto seen_key = [&](int key) { return key < span.end && (key >= span.lo || key < d.sinks); };
-  auto page_at = [&](int u, int at) {
-    if (u >= u1) return -1;
-    const int key = span.tile(u) * TN + at;
-    return seen_key(key) ? page_of(table, d.s.max_pages, d.c, key) : -1;
+  // The rows of a tile: thread i < TN finds key i's page two tiles before the
+  // loads need it and leaves its rows' offsets in LDS; -1 where nobody sees the
+  // key or it has no page.
+  int page_next = -1;
+  auto find_page = [&](int u) {
+    page_next = -1;
+    if (tid >= TN || u >= u1) return;
+    const int key = span.tile(u) * TN + tid;
+    if (key < span.end && (key >= span.lo || key < d.sinks)) page_next = page_of(table, d.s.max_pages, d.c, key);
   };
-  auto slot_of = [&](int key) { return key - fdiv(key, d.c.page_div) * d.c.page_size; };
+  auto find_rows = [&](int u) {
+    if (tid >= 64) return;
+    const int key = (u < u1 ? span.tile(u) * TN : 0) + tid;
+    const bool here = page_next >= 0;
+    const bool hole = tid < TN && u < u1 && !here && key < span.end && (key >= span.lo || key < d.sinks);
+    const uint64_t all = __ballot(here);
+    const bool holes = __any(hole);
+    if (tid == 0) seen_sh[u & 3] = all, hole_sh[u & 3] = holes;
+    if (tid >= TN) return;
+    const int64_t slot = key - fdiv(key, d.c.page_div) * d.c.page_size;
+    rows_sh[u & 3][0][tid] = here ? (page_next * d.c.k_page + slot * d.c.k_slot) * size : -1;
+    rows_sh[u & 3][1][tid] = here ? (page_next * d.c.v_page + slot * d.c.v_slot) * size : -1;
+  };
   u32x4 k_in[KL];
   uint32_t v_in[4][VW];
-  int k_page, v_page[4];
-  auto find_pages = [&](int u) {
-    k_page = page_at(u, k_row);
+  // (Past head_dim the row's last 16 bytes again: q is zero there, and those
+  // results are not stored.)
+  int k_at[KL];
 #pragma unroll
-    for (int r = 0; r < 4; r++) v_page[r] = page_at(u, v_key + r);
-  };
-  // The row in flight: a key that somebody sees; one that would be seen but
-  // has no page.
-  bool k_here, k_hole;
+  for (int j = 0; j < KL; j++) k_at[j] = min((8 * j + k_eighth) * PER, dim - PER) * size;
   auto load = [&](int u) {
-    const int base = u < u1 ? span.tile(u) * TN : 0;
-    k_here = k_page >= 0;
-    k_hole = u < u1 && !k_here && seen_key(base + k_row);
-    const char* kr = kc + ((int64_t)k_page * d.c.k_page + (int64_t)slot_of(base + k_row) * d.c.k_slot) * size;
+    const int64_t kr = rows_sh[u & 3][0][k_row];
 #pragma unroll
-    for (int j = 0; j < KL; j++) {
-      const int at = (8 * j + k_eighth) * PER;
-      k_in[j] = (u32x4){0, 0, 0, 0};
-      if (k_here && at < dim) k_in[j] = *(const u32x4*)(kr + at * size);
+    for (int j = 0; j < KL; j++) k_in[j] = (u32x4){0, 0, 0, 0};
+    if (kr >= 0) {
+#pragma unroll
+      for (int j = 0; j < KL; j++) k_in[j] = *(const u32x4*)(kc + kr + k_at[j]);
     }
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-      const char* vr = vc + ((int64_t)v_page[r] * d.c.v_page + (int64_t)slot_of(base + v_key + r) * d.c.v_slot) * size;
-      load_words<VW>(vr + v_group * DPV * size, v_page[r] >= 0 && v_group * DPV < dim, v_in[r]);
+      load_words<VW>(vc, rows_sh[u & 3][1][v_key + r], v_group * DPV * size, dim * size, v_in[r]);
     }
   };
   // What the conversion of the tile in the registers has to know of all of it.
@@ -864,16 +886,13 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
       v_top = wave_max(v_top);
       if (lane == 0) top_sh[parity][0][wave] = k_top, top_sh[parity][1][wave] = v_top;
     }
-    const bool hole = __any(k_hole);
-    if (lane == 0) hole_sh[parity][wave] = hole;
-    if (k_eighth == 0) seen_sh[u & 3][k_row] = k_here;
   };
 
   float m, l;
   f32x16 o[NB];
   int o_up;                         // o is 2^o_up times the result
   int k_up = 0, v_up;               // exponents of the tile converted last
-  bool holes = false, poison;
+  bool poison;
   // Converts the tile in the registers into its buffer.
   auto stage = [&](int parity) {
     float k_f = 1.f, v_f = 1.f;
@@ -882,15 +901,12 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
 #pragma unroll
       for (int i = 0; i < WAVES; i++)
         k_top = fmaxf(k_top, top_sh[parity][0][i]), v_top = fmaxf(v_top, top_sh[parity][1][i]);
-      k_up = exponent_for(k_top);
-      const int up = exponent_for(v_top);
+      k_up = __builtin_amdgcn_readfirstlane(exponent_for(k_top));
+      const int up = __builtin_amdgcn_readfirstlane(exponent_for(v_top));
       if (up < v_up) v_up = up - 1;  // larger values than any before: a binade more of room
       k_f = pow2(k_up);
       v_f = pow2(v_up);
     }
-    holes = false;
-#pragma unroll
-    for (int i = 0; i < WAVES; i++) holes |= hole_sh[parity][i] != 0;
     char* kt = &buffer_sh[parity][k_row * KS];
 #pragma unroll
     for (int j = 0; j < KL; j++) {
@@ -935,13 +951,11 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
       }
     }
   };
-  auto multiply = [&](int u, int k_exp, bool some_hole, bool careful) {
+  auto multiply = [&](int u, int k_exp, bool careful) {
     const int base = span.tile(u) * TN, parity = u & 1;
     // Tiles past all of the wave's rows, or before all their windows.
-    const int64_t below_lo = d.window ? (int64_t)pos_lo - d.window : -1;
-    if (!wave_ok || base > pos_hi || (d.window && base + TN - 1 <= below_lo && base >= d.sinks)) return;
-    const int64_t below_hi = d.window ? (int64_t)pos_hi - d.window : -1;
-    const bool whole = !some_hole && !careful && wave_row + 31 < all_rows && base + TN - 1 <= pos_lo &&
+    if (!wave_ok || base > pos_hi || (base + TN - 1 <= below_lo && base >= d.sinks)) return;
+    const bool whole = !__builtin_amdgcn_readfirstlane(hole_sh[u & 3]) && !careful && wave_row + 31 < all_rows && base + TN - 1 <= pos_lo &&
                        base + TN <= span.end && (base > below_hi || base + TN <= d.sinks);
     const float back = pow2(-q_up - k_exp);
     const char* ks = buffer_sh[parity];
@@ -966,11 +980,11 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
           const int in = 32 * tb + 2 * e + 4 * h, at = base + in;
-          const uint32_t here = *(const uint32_t*)&seen_sh[u & 3][in];
+          const uint32_t here = (uint32_t)(seen_sh[u & 3] >> in);
           const uint32_t bad = careful ? *(const uint32_t*)&bad_sh[u & 3][in] : 0;
 #pragma unroll
           for (int r = 0; r < 4; r++) {
-            const bool seen = (here >> (8 * r) & 1) && at + r <= pos && (at + r > below || at + r < d.sinks);
+            const bool seen = (here >> r & 1) && at + r <= pos && (at + r > below || at + r < d.sinks);
             if (!seen) s[e + r] = NEG_INF;
             poison |= seen && (bad >> (8 * r) & 1);
           }
@@ -1009,7 +1023,7 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
       for (int c = 0; c < 2; c++)
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-          const int at = value_at<TN>(32 * b + n, 2 * (2 * tb + c) + h);
+          const int at = (v_base ^ value_flip<TN>(32 * b, 2 * (2 * tb + c))) + 32 * b * TN * 2;
           const f16x8 a = *(const f16x8*)(vs + at);
           o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p_hi[c], o[b], 0, 0, 0);
           o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p_lo[c], o[b], 0, 0, 0);
@@ -1029,24 +1043,29 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
     for (int b = 0; b < NB; b++)
 #pragma unroll
       for (int e = 0; e < 16; e++) o[b][e] = 0.f;
-    find_pages(u0);
+    find_page(u0);
+    find_rows(u0);
+    find_page(u0 + 1);
+    find_rows(u0 + 1);
+    find_page(u0 + 2);
+    __syncthreads();
     load(u0);
-    find_pages(u0 + 1);
     measure(u0, careful);
+    find_rows(u0 + 2);
+    find_page(u0 + 3);
     __syncthreads();
     stage(u0 & 1);
     load(u0 + 1);
-    find_pages(u0 + 2);
     measure(u0 + 1, careful);
     for (int u = u0; u < u1; u++) {
       const int k_exp = k_up, v_exp = v_up;
-      const bool some_hole = holes;
-      // Tile u is in its buffer, u + 1's tops are there, and nobody reads
-      // u - 1 any more.
+      // Tile u is in its buffer, u + 1's tops and u + 2's rows are there, and
+      // nobody reads u - 1 any more.
       __syncthreads();
       if (u + 1 < u1) stage((u + 1) & 1);
       load(u + 2);
-      find_pages(u + 3);
+      find_rows(u + 3);
+      find_page(u + 4);
       if (SCALED && v_exp != o_up) {
         const float f = pow2(v_exp - o_up);
         o_up = v_exp;
@@ -1055,7 +1074,7 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
 #pragma unroll
           for (int e = 0; e < 16; e++) o[b][e] *= f;
       }
-      multiply(u, k_exp, some_hole, careful);
+      multiply(u, k_exp, careful);
       measure(u + 2, careful);
     }
     __syncthreads();
@@ -1091,11 +1110,6 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
 
 // ---- merge ---------------------------------------------------------------------------
 
-// out = sum_i l_i 2^(m_i - max m) o_i / sum_i l_i 2^(m_i - max m) over the
-// stretches of a tile.  A tile's numbers are joined 64 at a time, by 16
-// threads for each four of them that take every 16th stretch; the tile's
-// stretches, which are as many slots, divide those 64s among themselves, so a
-// tile of many stretches is joined by many workgroups.
 __device__ __forceinline__ void join(float& m, float& l, f32x4& o, float m2, float l2, const f32x4& o2) {
   const float top = fmaxf(m, m2), ref = top == NEG_INF ? 0.f : top;
   const float a = __builtin_amdgcn_exp2f(m - ref), b = __builtin_amdgcn_exp2f(m2 - ref);
@@ -1106,28 +1120,45 @@ __device__ __forceinline__ void join(float& m, float& l, f32x4& o, float m2, flo
 }
 
 constexpr int PA_MERGE_GRID = 512;
+constexpr int PA_MERGE_BIG = 32;    // waves for a stretch's share of a chunk tile
+constexpr int PA_MERGE_LEAST = 4;   // 16-byte pieces of a share
 
+// out = sum_i l_i 2^(m_i - max m) o_i / sum_i l_i 2^(m_i - max m) over the
+// stretches of a tile.  The stretches, which are as many slots, divide the
+// tile's numbers among themselves, so a tile of many stretches is joined by
+// many waves; where a share is short, several lanes take the stretches of a
+// piece between them.  Bound by the latency of three dependent loads.
 __global__ __launch_bounds__(PA_THREADS) void merge_kernel(PagedDesc d) {
-  __shared__ float m_sh[4][16], l_sh[4][16];
-  __shared__ f32x4 o_sh[4][16];
-  const int n_small = d.slots_small ? d.slots[0] : 0, n_all = n_small + (d.slots_big ? d.slots[1] : 0);
-  const int tid = threadIdx.x, col = tid & 15, first = tid >> 4, wave = tid >> 6;
+  const int n_small = d.slots_small ? d.slots[0] : 0, n_big = d.slots_big ? d.slots[1] : 0;
+  const int units = n_small + n_big * PA_MERGE_BIG;
+  const int lane = threadIdx.x & 63;
   const int dim = d.c.dim, quads = dim / 4;
-  for (int s = blockIdx.x; s < n_all; s += gridDim.x) {
-    const bool big = s >= n_small;
-    const Part p = big ? d.part_big[s - n_small] : d.part_small[s];
+  for (int unit = blockIdx.x * (PA_THREADS / 64) + (threadIdx.x >> 6); unit < units;
+       unit += gridDim.x * (PA_THREADS / 64)) {
+    const bool big = unit >= n_small;
+    const int at_big = unit - n_small;
+    const Part p = big ? d.part_big[at_big / PA_MERGE_BIG] : d.part_small[unit];
     const float* os = big ? d.o_big : d.o_small;
     const float2* ml = big ? d.ml_big : d.ml_small;
     const int tile_rows = big ? d.rows_big : PA_SMALL;
     const int slot0 = p.slot - p.part * p.stride;
     const int n = p.rows * quads;
-    for (int c0 = p.part * 16; c0 < n; c0 += p.parts * 16) {
-      const int at = c0 + col;
-      const int row = min(at, n - 1) / quads, c = (min(at, n - 1) - row * quads) * 4;
+    const int shares = big ? p.parts * PA_MERGE_BIG : p.parts;
+    const int share = big ? p.part * PA_MERGE_BIG + at_big % PA_MERGE_BIG : p.part;
+    const int each = max(PA_MERGE_LEAST, (n + shares - 1) / shares);
+    const int begin = min(n, share * each), end = min(n, begin + each);
+    if (begin >= end) continue;
+    // Lanes for a piece: as many as leave a lane for every piece of the share.
+    int lanes = 64;
+    while (lanes > 1 && lanes * (end - begin) > 64) lanes >>= 1;
+    const int first = lane & (lanes - 1);
+    for (int at0 = begin; at0 < end; at0 += 64 / lanes) {
+      const int at = at0 + lane / lanes, in = min(at, end - 1);
+      const int row = in / quads, c = (in - row * quads) * 4;
       float m = NEG_INF, l = 0.f;
       f32x4 o = {0, 0, 0, 0};
 #pragma unroll 4
-      for (int i = first; i < p.parts; i += 16) {
+      for (int i = first; i < p.parts; i += lanes) {
         const int64_t at_row = (slot0 + (int64_t)i * p.stride) * tile_rows + row;
         const float2 x = ml[at_row];
         f32x4 y = *(const f32x4*)(os + at_row * dim + c);
@@ -1135,25 +1166,20 @@ __global__ __launch_bounds__(PA_THREADS) void merge_kernel(PagedDesc d) {
         for (int e = 0; e < 4; e++) y[e] = x.y == 0.f ? 0.f : y[e] * x.y;
         join(m, l, o, x.x, x.y, y);
       }
-#pragma unroll
-      for (int k = 16; k < 64; k <<= 1) {
+      for (int k = 1; k < lanes; k <<= 1) {
         f32x4 y;
 #pragma unroll
         for (int e = 0; e < 4; e++) y[e] = __shfl_xor(o[e], k);
-        join(m, l, o, __shfl_xor(m, k), __shfl_xor(l, k), y);
+        const float m2 = __shfl_xor(m, k), l2 = __shfl_xor(l, k);
+        join(m, l, o, m2, l2, y);
       }
-      if ((first & 3) == 0) m_sh[wave][col] = m, l_sh[wave][col] = l, o_sh[wave][col] = o;
-      __syncthreads();
-      if (tid < 16 && at < n) {
-#pragma unroll
-        for (int k = 1; k < 4; k++) join(m, l, o, m_sh[k][col], l_sh[k][col], o_sh[k][col]);
+      if (first == 0 && at < end) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
         for (int e = 0; e < 4; e++) o[e] *= inv;
         const int r = p.row0 + row, token = fdiv(r, d.group_div), sub = r - token * d.group;
         *(f32x4*)(d.out + (int64_t)(p.token0 + token) * d.o_t + (int64_t)(p.head * d.group + sub) * d.o_h + c) = o;
       }
-      __syncthreads();
     }
   }
 }

@@ -307,6 +307,16 @@ def test_attention_chunks(rh, cache_type, hq, hk, dim, q_lens, kv_lens, page):
 
 
 @pytest.mark.parametrize("cache_type", TYPES)
+@pytest.mark.parametrize("dim", [16, 24, 56, 72, 104, 136, 152, 200, 248])
+def test_attention_odd_head_dims(rh, cache_type, dim):
+    for q_lens, kv_lens in (([1, 1], [70, 9]), ([30, 1], [100, 9])):
+        s = Paged(q_lens, kv_lens, 16)
+        got, q, k, v, scale = run_attention(rh, s, 4, 2, dim, cache_type)
+        want, tol = attention_ref(q, k, v, s, scale, 0, 0)
+        attention_close(got, want, tol)
+
+
+@pytest.mark.parametrize("cache_type", TYPES)
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 3), (17, 0), (64, 4), (100, 70), (1000, 4), (2 ** 31 - 1, 2 ** 31 - 1)])
 @pytest.mark.parametrize("q_lens,kv_lens", [([1, 1, 1], [500, 64, 3]), ([40, 3], [333, 70])])
 def test_attention_window(rh, cache_type, window, sinks, q_lens, kv_lens):
