@@ -520,7 +520,7 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         const int at = base + r;
-        seen[r] = here[r] && at <= pos && (at > below || at < d.sinks);
+        seen[r] = here[r] & (at <= pos) & ((at > below) | (at < d.sinks));
         p[r] = seen[r] ? (s0[r] + s1[r]) * q_back : NEG_INF;
         top = fmaxf(top, p[r]);
       }
@@ -731,12 +731,41 @@ __device__ __forceinline__ float top_of(float top, uint32_t w) {
   return fmaxf(top, fmaxf(fabsf(cache_lo<TYPE>(w)), fabsf(cache_hi<TYPE>(w))));
 }
 
+// x, of which the compiler does not know that it is the same in every round of
+// a loop: what follows from it is formed again there, a few instructions,
+// instead of being held in a register that the products' operands need.
+__device__ __forceinline__ int afresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// Steps 0 .. STEPS - 1, each reading its operands from LDS (read) and then
+// multiplying them (multiply): the reads are AHEAD steps before the products,
+// which the compiler, short of registers, would put right behind them.
+template <int STEPS, int AHEAD, typename Operands, typename Read, typename Multiply>
+__device__ __forceinline__ void pipelined(Read read, Multiply multiply) {
+  Operands x[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; i++) x[i] = read(i);
+#pragma unroll
+  for (int i = 0; i < STEPS; i++) {
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(i, x[i % AHEAD]);
+    __builtin_amdgcn_sched_barrier(0);
+    if (i + AHEAD < STEPS) x[i % AHEAD] = read(i + AHEAD);
+  }
+}
+
 template <int DP, int TYPE>
 __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) void chunk_kernel(PagedDesc d) {
   using T = ChunkTile<DP, TYPE>;
   constexpr int TERMS = T::TERMS, KS = T::KS, KL = T::KL, VW = T::VW, DPV = T::DPV, TN = T::TN, WAVES = T::WAVES;
   constexpr int size = CacheType<TYPE>::size, PER = 16 / size, NB = DP / 32;
   constexpr bool SCALED = TYPE != RTENHIP_CACHE_F16;  // f16 rows go to LDS as they are
+  constexpr int AHEAD = 2;  // LDS reads before their products, in steps
+  struct Operands {
+    f16x8 term[TERMS];
+  };
   __shared__ PlanShared plan_sh;
   __shared__ __attribute__((aligned(16))) char buffer_sh[2][T::BUFFER];  // keys hi, lo, values hi, lo
   __shared__ float top_sh[2][2][WAVES];                                  // [tile & 1][keys, values]
@@ -745,7 +774,7 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
   __shared__ int64_t rows_sh[4][2][TN];
   __shared__ uint64_t seen_sh[4];
   __shared__ int hole_sh[4];
-  __shared__ __attribute__((aligned(4))) uint8_t bad_sh[4][TN];
+  __shared__ uint64_t bad_sh[4];
   Work w;
   if (!plan<true, T::THREADS, T::ROWS>(d, blockIdx.x, plan_sh, w) || w.slot >= d.slots_big) return;
   const int row0 = w.tile * T::ROWS;
@@ -809,9 +838,12 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
 
   // Staging: keys, thread (row, eighth of it); values, thread (4 keys, DP / 32
   // dimensions), the two halves of a wave on the two halves of a chunk.
-  const int k_row = tid >> 3, k_eighth = tid & 7, v_group = tid & 31;
-  const int v_chunk = (tid >> 7) * 2 + (tid >> 6 & 1), v_half = tid >> 5 & 1;
-  const int v_key = 16 * (tid >> 7) + 8 * v_half + 4 * (tid >> 6 & 1);
+  struct Place {
+    int k_row, k_eighth, v_group, v_chunk, v_half, v_key;
+    __device__ explicit Place(int t)
+        : k_row(t >> 3), k_eighth(t & 7), v_group(t & 31), v_chunk((t >> 7) * 2 + (t >> 6 & 1)), v_half(t >> 5 & 1),
+          v_key(16 * (t >> 7) + 8 * (t >> 5 & 1) + 4 * (t >> 6 & 1)) {}
+  };
   // The rows of a tile: thread i < TN finds key i's page two tiles before the
   // loads need it and leaves its rows' offsets in LDS; -1 where nobody sees the
   // key or it has no page.
@@ -829,7 +861,7 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
     const bool hole = tid < TN && u < u1 && !here && key < span.end && (key >= span.lo || key < d.sinks);
     const uint64_t all = __ballot(here);
     const bool holes = __any(hole);
-    if (tid == 0) seen_sh[u & 3] = all, hole_sh[u & 3] = holes;
+    if (tid == 0) seen_sh[u & 3] = all, hole_sh[u & 3] = holes, bad_sh[u & 3] = 0;
     if (tid >= TN) return;
     const int64_t slot = key - fdiv(key, d.c.page_div) * d.c.page_size;
     rows_sh[u & 3][0][tid] = here ? (page_next * d.c.k_page + slot * d.c.k_slot) * size : -1;
@@ -839,21 +871,19 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
   uint32_t v_in[4][VW];
   // (Past head_dim the row's last 16 bytes again: q is zero there, and those
   // results are not stored.)
-  int k_at[KL];
-#pragma unroll
-  for (int j = 0; j < KL; j++) k_at[j] = min((8 * j + k_eighth) * PER, dim - PER) * size;
   auto load = [&](int u) {
-    const int64_t kr = rows_sh[u & 3][0][k_row];
+    const Place at(afresh(tid));
+    const int64_t kr = rows_sh[u & 3][0][at.k_row];
 #pragma unroll
     for (int j = 0; j < KL; j++) k_in[j] = (u32x4){0, 0, 0, 0};
     if (kr >= 0) {
 #pragma unroll
-      for (int j = 0; j < KL; j++) k_in[j] = *(const u32x4*)(kc + kr + k_at[j]);
+      for (int j = 0; j < KL; j++)
+        k_in[j] = *(const u32x4*)(kc + kr + min((8 * j + at.k_eighth) * PER, dim - PER) * size);
     }
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-      load_words<VW>(vc, rows_sh[u & 3][1][v_key + r], v_group * DPV * size, dim * size, v_in[r]);
-    }
+    for (int r = 0; r < 4; r++)
+      load_words<VW>(vc, rows_sh[u & 3][1][at.v_key + r], at.v_group * DPV * size, dim * size, v_in[r]);
   };
   // What the conversion of the tile in the registers has to know of all of it.
   auto measure = [&](int u, bool careful) {
@@ -864,8 +894,7 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
         bool bad = false;
 #pragma unroll
         for (int c = 0; c < VW; c++) bad |= clean<TYPE>(v_in[r][c]);
-        const uint64_t all = __ballot(bad);  // (a key's values are in one half of the wave)
-        if (v_group == 0) bad_sh[u & 3][v_key + r] = (uint32_t)(all >> (lane & 32)) != 0;
+        if (bad) atomicOr((unsigned long long*)&bad_sh[u & 3], 1ull << (Place(tid).v_key + r));
       }
     }
     if constexpr (SCALED) {
@@ -907,10 +936,11 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
       k_f = pow2(k_up);
       v_f = pow2(v_up);
     }
-    char* kt = &buffer_sh[parity][k_row * KS];
+    const Place p(afresh(tid));
+    char* kt = &buffer_sh[parity][p.k_row * KS];
 #pragma unroll
     for (int j = 0; j < KL; j++) {
-      const int at = (8 * j + k_eighth) * PER * 2;
+      const int at = (8 * j + p.k_eighth) * PER * 2;
       if constexpr (TYPE == RTENHIP_CACHE_F16) {
         *(u32x4*)(kt + at) = k_in[j];
       } else if constexpr (TYPE == RTENHIP_CACHE_BF16) {
@@ -928,10 +958,10 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
         *(f16x4*)(kt + T::K_BYTES + at) = (f16x4){l0[0], l0[1], l1[0], l1[1]};
       }
     }
-    char* vt = &buffer_sh[parity][TERMS * T::K_BYTES + 8 * v_half];
+    char* vt = &buffer_sh[parity][TERMS * T::K_BYTES + 8 * p.v_half];
 #pragma unroll
     for (int e = 0; e < DPV; e++) {
-      const int at = value_at<TN>(DPV * v_group + e, v_chunk);
+      const int at = value_at<TN>(DPV * p.v_group + e, p.v_chunk);
       if constexpr (TYPE == RTENHIP_CACHE_F16) {
         const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
         *(u32x2*)(vt + at) = (u32x2){__builtin_amdgcn_perm(v_in[1][e / 2], v_in[0][e / 2], sel),
@@ -966,29 +996,32 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
 #pragma unroll
       for (int e = 0; e < 16; e++) s[e] = 0.f;
       const char* kr = ks + (32 * tb + n) * KS + 16 * h;
+      pipelined<DP / 16, AHEAD, Operands>(
+          [&](int j) {
+            Operands x;
 #pragma unroll
-      for (int j = 0; j < DP / 16; j++) {
-        const f16x8 a = *(const f16x8*)(kr + 32 * j);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q_hi[j], s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q_lo[j], s, 0, 0, 0);
-        if constexpr (TERMS == 2) {
-          const f16x8 b = *(const f16x8*)(kr + T::K_BYTES + 32 * j);
-          s = __builtin_amdgcn_mfma_f32_32x32x16_f16(b, q_hi[j], s, 0, 0, 0);
-        }
-      }
+            for (int i = 0; i < TERMS; i++) x.term[i] = *(const f16x8*)(kr + i * T::K_BYTES + 32 * j);
+            return x;
+          },
+          [&](int j, const Operands& x) {
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.term[0], q_hi[j], s, 0, 0, 0);
+            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.term[0], q_lo[j], s, 0, 0, 0);
+            if constexpr (TERMS == 2) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.term[1], q_hi[j], s, 0, 0, 0);
+          });
       if (!whole) {
+        // (Without short circuits: a branch for each score costs the registers
+        // of several copies of s.)
+        const int in = 32 * tb + 4 * (afresh(lane) >> 5), at = base + in;
+        const uint32_t here = (uint32_t)(seen_sh[u & 3] >> in);
+        uint32_t seen = 0;
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const int in = 32 * tb + 2 * e + 4 * h, at = base + in;
-          const uint32_t here = (uint32_t)(seen_sh[u & 3] >> in);
-          const uint32_t bad = careful ? *(const uint32_t*)&bad_sh[u & 3][in] : 0;
-#pragma unroll
-          for (int r = 0; r < 4; r++) {
-            const bool seen = (here >> r & 1) && at + r <= pos && (at + r > below || at + r < d.sinks);
-            if (!seen) s[e + r] = NEG_INF;
-            poison |= seen && (bad >> (8 * r) & 1);
-          }
+        for (int e = 0; e < 16; e++) {
+          const int k = (e & 3) + 8 * (e >> 2);  // at + k: the key of s[e]
+          const bool ok = (here >> k & 1) & (at + k <= pos) & ((at + k > below) | (at + k < d.sinks));
+          s[e] = ok ? s[e] : NEG_INF;
+          seen |= (uint32_t)ok << k;
         }
+        if (careful) poison |= (seen & (uint32_t)(bad_sh[u & 3] >> in)) != 0;
       }
       float top = s[0];
 #pragma unroll
@@ -1019,19 +1052,21 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
         p_lo[e >> 3][e & 7] = lo[0], p_lo[e >> 3][(e & 7) + 1] = lo[1];
       }
       l += sum;
+      pipelined<2 * NB, AHEAD, Operands>(
+          [&](int i) {
+            const int c = i / NB, b = i % NB;
+            const int at = (v_base ^ value_flip<TN>(32 * b, 2 * (2 * tb + c))) + 32 * b * TN * 2;
+            Operands x;
 #pragma unroll
-      for (int c = 0; c < 2; c++)
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-          const int at = (v_base ^ value_flip<TN>(32 * b, 2 * (2 * tb + c))) + 32 * b * TN * 2;
-          const f16x8 a = *(const f16x8*)(vs + at);
-          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p_hi[c], o[b], 0, 0, 0);
-          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p_lo[c], o[b], 0, 0, 0);
-          if constexpr (TERMS == 2) {
-            const f16x8 z = *(const f16x8*)(vs + T::V_BYTES + at);
-            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(z, p_hi[c], o[b], 0, 0, 0);
-          }
-        }
+            for (int k = 0; k < TERMS; k++) x.term[k] = *(const f16x8*)(vs + k * T::V_BYTES + at);
+            return x;
+          },
+          [&](int i, const Operands& x) {
+            const int c = i / NB, b = i % NB;
+            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.term[0], p_hi[c], o[b], 0, 0, 0);
+            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.term[0], p_lo[c], o[b], 0, 0, 0);
+            if constexpr (TERMS == 2) o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.term[1], p_hi[c], o[b], 0, 0, 0);
+          });
     }
   };
   // A tile's buffer, tops and flags go by the parity of its number.
@@ -1093,8 +1128,8 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
   if (!row_ok) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const float v_back = SCALED ? pow2(-o_up) : 1.f;
-  const int r = wave * 32 + n;
-  float* to = w.slot < 0 ? d.out + (int64_t)(w.start + token) * d.o_t + (int64_t)(w.head * d.group + sub) * d.o_h
+  const int r = afresh(wave * 32 + n), to_token = fdiv(row0 + r, d.group_div), to_sub = row0 + r - to_token * d.group;
+  float* to = w.slot < 0 ? d.out + (int64_t)(w.start + to_token) * d.o_t + (int64_t)(w.head * d.group + to_sub) * d.o_h
                          : d.o_big + ((int64_t)w.slot * T::ROWS + r) * dim;
   if (w.slot >= 0 && h == 0) d.ml_big[(int64_t)w.slot * T::ROWS + r] = make_float2(m, l);
 #pragma unroll
