@@ -243,15 +243,21 @@ __device__ __forceinline__ float quarter_sum(float x) {
   return half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 template <int CTRL>
-__device__ __forceinline__ float dpp(float x) {
-  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xF, 0xF, true));
+__device__ __forceinline__ uint32_t max_dpp(uint32_t x) {
+  return max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xF, 0xF, true));
 }
-__device__ __forceinline__ float wave_max(float x) {
-  x = fmaxf(x, dpp<0xB1>(x));   // lane ^ 1
-  x = fmaxf(x, dpp<0x4E>(x));   // lane ^ 2
-  x = fmaxf(x, dpp<0x141>(x));  // mirrored in its 8
-  x = fmaxf(x, dpp<0x140>(x));  // mirrored in its 16
-  return quarter_max(x);
+// The largest of the wave's numbers, none negative (their bits are in the
+// same order).
+__device__ __forceinline__ float wave_max(float y) {
+  uint32_t x = __float_as_uint(y);
+  x = max_dpp<0xB1>(x);   // lane ^ 1
+  x = max_dpp<0x4E>(x);   // lane ^ 2
+  x = max_dpp<0x141>(x);  // mirrored in its 8
+  x = max_dpp<0x140>(x);  // mirrored in its 16
+  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = max(r[0], r[1]);
+  const auto s = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return __uint_as_float(max(s[0], s[1]));
 }
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
@@ -269,12 +275,27 @@ __device__ __forceinline__ float pow2(int e) {  // e brought into the normal ran
   return __uint_as_float((uint32_t)(e + 127) << 23);
 }
 
+// x, of which the compiler does not know where it comes from (no instruction).
+template <typename T>
+__device__ __forceinline__ T opaque(T x) {
+  static_assert(sizeof(T) == 4, "one register");
+  asm("" : "+v"(x));
+  return x;
+}
+
 // x = hi + lo in f16: 22 bits of x where |x| is within 2^14 and above 2^-3,
-// an absolute error of 2^-25 below that.  lo is x - hi exactly (one mixed
-// fma, hi times the -1 that is a register, before its own rounding).
+// an absolute error of 2^-25 below that.  lo is x - hi exactly, by one mixed
+// fma that reads hi from its half of the register, before its own rounding:
+// the -1 has to be a register for that, and hi not be seen to be a conversion,
+// which would be repeated for each half.
 __device__ __forceinline__ void split16(float a, float b, float minus1, f16x2& hi, f16x2& lo) {
-  hi = (f16x2){(_Float16)a, (_Float16)b};
+  hi = opaque((f16x2){(_Float16)a, (_Float16)b});
   lo = (f16x2){(_Float16)__builtin_fmaf((float)hi[0], minus1, a), (_Float16)__builtin_fmaf((float)hi[1], minus1, b)};
+}
+// The same of a f and b f, f a power of two.
+__device__ __forceinline__ void split16(float a, float b, float f, float minus1, f16x2& hi, f16x2& lo) {
+  hi = opaque((f16x2){(_Float16)(a * f), (_Float16)(b * f)});
+  lo = (f16x2){(_Float16)__builtin_fmaf(a, f, -(float)hi[0]), (_Float16)__builtin_fmaf(b, f, -(float)hi[1])};
 }
 
 template <int TYPE>
@@ -659,10 +680,11 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
 //  - an f32 number x 2^e is hi + lo, each f16 (split16), and a product
 //    hi hi + hi lo + lo hi, three f16 instructions against the eight times
 //    longer f32 one, loses what is below 2^-22 of it; a 16-bit cache needs no
-//    lo.  e is one power of two for the tile's keys and one, which only ever
-//    falls, for the values so far, so the largest number of either is near
-//    2^13 and the terms are exact to 2^-38 of it; q has one for each row, p
-//    the factor 2^8.  Powers of two come out again exactly.
+//    lo.  e is one power of two for every 8 keys and one for their values, so
+//    that the largest number of either is near 2^13 and the terms are exact to
+//    2^-38 of it; q has one for each row, p the factor 2^8.  Powers of two come
+//    out again exactly: a score is multiplied by its keys' and its row's on
+//    its way into the exponential, whose argument takes the values'.
 //  - S^T = K Q^T: a lane (n, h) has row n's scores for the keys
 //    8 i + 4 h + j of each 32, so the softmax needs one exchange with lane
 //    ^ 32, and
@@ -672,10 +694,11 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
 //  is passed by more than 2^6, which few tiles do, so the result is hardly
 //  ever rescaled.
 // Two LDS buffers and one barrier a tile: while tile u is multiplied, u + 1 is
-// converted into the other buffer and u + 2 is on its way into registers.
-// Eight waves, two to a SIMD, so that one's conversions and exponentials run
-// under the other's products; at head_dim 256 a wave needs all of a SIMD's
-// registers, and four waves work on tiles of 32 keys.
+// converted into the other buffer, 8 keys by each wave, and u + 2 is on its way
+// into registers.  Eight waves, two to a SIMD: one of the two converts before
+// it multiplies and the other after, which keeps one's conversions and
+// exponentials under the other's products; at head_dim 256 a wave needs all of
+// a SIMD's registers, and four waves work on tiles of 32 keys.
 // Bound by the matrix instructions at long prompts.
 template <int DP, int TYPE>
 struct ChunkTile {
@@ -724,12 +747,26 @@ __device__ __forceinline__ float cache_hi(uint32_t w) {
   return __uint_as_float(w & 0xffff0000u);
 }
 
-// The largest magnitude in a word of the cache and `top`.
+// The largest magnitude among `top` and two words of the cache; a NaN counts as
+// nothing.  (The instruction takes magnitudes as it goes; fmaxf would first
+// quiet what comes from memory.)
 template <int TYPE>
-__device__ __forceinline__ float top_of(float top, uint32_t w) {
-  if constexpr (TYPE == RTENHIP_CACHE_F32) return fmaxf(top, fabsf(__uint_as_float(w)));
-  return fmaxf(top, fmaxf(fabsf(cache_lo<TYPE>(w)), fabsf(cache_hi<TYPE>(w))));
+__device__ __forceinline__ float top_of(float top, uint32_t x, uint32_t y) {
+  const auto max3 = [](float a, float b, float c) {
+    asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(a) : "v"(a), "v"(b), "v"(c));
+    return a;
+  };
+  if constexpr (TYPE == RTENHIP_CACHE_F32) return max3(top, __uint_as_float(x), __uint_as_float(y));
+  return max3(max3(top, cache_lo<TYPE>(x), cache_hi<TYPE>(x)), cache_lo<TYPE>(y), cache_hi<TYPE>(y));
 }
+
+// What is known of a tile in LDS: the exponents of every 8 keys and of their
+// values, and by bits the keys that somebody sees and those with a value that
+// is not finite.
+struct __attribute__((aligned(16))) TileInfo {
+  int8_t k_up[8], v_up[8];
+  uint64_t seen, bad;
+};
 
 // x, of which the compiler does not know that it is the same in every round of
 // a loop: what follows from it is formed again there, a few instructions,
@@ -768,13 +805,9 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
   };
   __shared__ PlanShared plan_sh;
   __shared__ __attribute__((aligned(16))) char buffer_sh[2][T::BUFFER];  // keys hi, lo, values hi, lo
-  __shared__ float top_sh[2][2][WAVES];                                  // [tile & 1][keys, values]
-  // [tile & 3], as they are read late: the keys' rows [keys, values], those
-  // that somebody sees, whether one lacks its page, whose value is not finite.
-  __shared__ int64_t rows_sh[4][2][TN];
-  __shared__ uint64_t seen_sh[4];
-  __shared__ int hole_sh[4];
-  __shared__ uint64_t bad_sh[4];
+  // [tile & 3], as they are read late.
+  __shared__ int64_t rows_sh[4][2][TN];  // the keys' and the values' rows
+  __shared__ TileInfo info_sh[4];
   Work w;
   if (!plan<true, T::THREADS, T::ROWS>(d, blockIdx.x, plan_sh, w) || w.slot >= d.slots_big) return;
   const int row0 = w.tile * T::ROWS;
@@ -798,7 +831,7 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
   const int below_lo = sinks_only(d, pos_lo), below_hi = sinks_only(d, pos_hi);
 
   f16x8 q_hi[DP / 16], q_lo[DP / 16];
-  int q_up;
+  float q_back;  // 1 / the row's power of two
   {
     const float* q = d.q + (int64_t)(w.start + token) * d.q_t + (int64_t)(w.head * d.group + sub) * d.q_h;
     float x[DP / 16][8], top = 0.f;
@@ -815,8 +848,9 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
 #pragma unroll
       for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[j][e]));
     }
-    q_up = exponent_for(half_max(top));
+    const int q_up = exponent_for(half_max(top));
     const float f = pow2(q_up);
+    q_back = pow2(-q_up);
 #pragma unroll
     for (int j = 0; j < DP / 16; j++)
 #pragma unroll
@@ -836,32 +870,31 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
   const char* kc = d.c.k + (int64_t)w.head * d.c.k_head * size;
   const char* vc = d.c.v + (int64_t)w.head * d.c.v_head * size;
 
-  // Staging: keys, thread (row, eighth of it); values, thread (4 keys, DP / 32
-  // dimensions), the two halves of a wave on the two halves of a chunk.
+  // Staging: wave w has keys 8 w .. 8 w + 7 of the tile, i = w & 1 of their 16;
+  // of the keys a thread has an eighth of a row, of the values DP / 32
+  // dimensions of four rows (h = half of the wave).
   struct Place {
     int k_row, k_eighth, v_group, v_chunk, v_half, v_key;
     __device__ explicit Place(int t)
-        : k_row(t >> 3), k_eighth(t & 7), v_group(t & 31), v_chunk((t >> 7) * 2 + (t >> 6 & 1)), v_half(t >> 5 & 1),
-          v_key(16 * (t >> 7) + 8 * (t >> 5 & 1) + 4 * (t >> 6 & 1)) {}
+        : k_row(t >> 3), k_eighth(t & 7), v_group(t & 31), v_chunk((t >> 7) * 2 + (t >> 5 & 1)), v_half(t >> 6 & 1),
+          v_key(t >> 5 << 2) {}
   };
   // The rows of a tile: thread i < TN finds key i's page two tiles before the
   // loads need it and leaves its rows' offsets in LDS; -1 where nobody sees the
   // key or it has no page.
   int page_next = -1;
-  auto find_page = [&](int u) {
+  auto find_page = [&](int u) __attribute__((always_inline)) {
     page_next = -1;
     if (tid >= TN || u >= u1) return;
     const int key = span.tile(u) * TN + tid;
     if (key < span.end && (key >= span.lo || key < d.sinks)) page_next = page_of(table, d.s.max_pages, d.c, key);
   };
-  auto find_rows = [&](int u) {
+  auto find_rows = [&](int u) __attribute__((always_inline)) {
     if (tid >= 64) return;
     const int key = (u < u1 ? span.tile(u) * TN : 0) + tid;
     const bool here = page_next >= 0;
-    const bool hole = tid < TN && u < u1 && !here && key < span.end && (key >= span.lo || key < d.sinks);
     const uint64_t all = __ballot(here);
-    const bool holes = __any(hole);
-    if (tid == 0) seen_sh[u & 3] = all, hole_sh[u & 3] = holes, bad_sh[u & 3] = 0;
+    if (tid == 0) info_sh[u & 3].seen = all, info_sh[u & 3].bad = 0;
     if (tid >= TN) return;
     const int64_t slot = key - fdiv(key, d.c.page_div) * d.c.page_size;
     rows_sh[u & 3][0][tid] = here ? (page_next * d.c.k_page + slot * d.c.k_slot) * size : -1;
@@ -871,7 +904,7 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
   uint32_t v_in[4][VW];
   // (Past head_dim the row's last 16 bytes again: q is zero there, and those
   // results are not stored.)
-  auto load = [&](int u) {
+  auto load = [&](int u) __attribute__((always_inline)) {
     const Place at(afresh(tid));
     const int64_t kr = rows_sh[u & 3][0][at.k_row];
 #pragma unroll
@@ -885,8 +918,12 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
     for (int r = 0; r < 4; r++)
       load_words<VW>(vc, rows_sh[u & 3][1][at.v_key + r], at.v_group * DPV * size, dim * size, v_in[r]);
   };
-  // What the conversion of the tile in the registers has to know of all of it.
-  auto measure = [&](int u, bool careful) {
+  float m, l;
+  f32x16 o[NB];
+  int o_up;  // o is 2^o_up times the result
+  bool poison;
+  // Converts the tile in the registers into its buffer.
+  auto stage = [&](int u, bool careful) __attribute__((always_inline)) {
     const int parity = u & 1;
     if (careful) {
 #pragma unroll
@@ -894,45 +931,35 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
         bool bad = false;
 #pragma unroll
         for (int c = 0; c < VW; c++) bad |= clean<TYPE>(v_in[r][c]);
-        if (bad) atomicOr((unsigned long long*)&bad_sh[u & 3], 1ull << (Place(tid).v_key + r));
+        if (bad) atomicOr((unsigned long long*)&info_sh[u & 3].bad, 1ull << (Place(tid).v_key + r));
       }
     }
-    if constexpr (SCALED) {
-      float k_top = 0.f, v_top = 0.f;
-#pragma unroll
-      for (int j = 0; j < KL; j++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          uint32_t x = k_in[j][e];
-          if (careful) clean<TYPE>(x);
-          k_top = top_of<TYPE>(k_top, x);
-        }
-#pragma unroll
-      for (int r = 0; r < 4; r++)
-#pragma unroll
-        for (int c = 0; c < VW; c++) v_top = top_of<TYPE>(v_top, v_in[r][c]);
-      k_top = wave_max(k_top);
-      v_top = wave_max(v_top);
-      if (lane == 0) top_sh[parity][0][wave] = k_top, top_sh[parity][1][wave] = v_top;
-    }
-  };
-
-  float m, l;
-  f32x16 o[NB];
-  int o_up;                         // o is 2^o_up times the result
-  int k_up = 0, v_up;               // exponents of the tile converted last
-  bool poison;
-  // Converts the tile in the registers into its buffer.
-  auto stage = [&](int parity) {
     float k_f = 1.f, v_f = 1.f;
     if constexpr (SCALED) {
       float k_top = 0.f, v_top = 0.f;
+      if (careful) {
 #pragma unroll
-      for (int i = 0; i < WAVES; i++)
-        k_top = fmaxf(k_top, top_sh[parity][0][i]), v_top = fmaxf(v_top, top_sh[parity][1][i]);
-      k_up = __builtin_amdgcn_readfirstlane(exponent_for(k_top));
-      const int up = __builtin_amdgcn_readfirstlane(exponent_for(v_top));
-      if (up < v_up) v_up = up - 1;  // larger values than any before: a binade more of room
+        for (int j = 0; j < KL; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            uint32_t x = k_in[j][e];
+            clean<TYPE>(x);
+            k_top = top_of<TYPE>(k_top, x, 0);
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < KL; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) k_top = top_of<TYPE>(k_top, k_in[j][e], k_in[j][e + 1]);
+      }
+#pragma unroll
+      for (int c = 0; c < VW; c++) {
+        v_top = top_of<TYPE>(v_top, v_in[0][c], v_in[1][c]);
+        v_top = top_of<TYPE>(v_top, v_in[2][c], v_in[3][c]);
+      }
+      const int k_up = __builtin_amdgcn_readfirstlane(exponent_for(wave_max(k_top)));
+      const int v_up = __builtin_amdgcn_readfirstlane(exponent_for(wave_max(v_top)));
+      if (lane == 0) info_sh[u & 3].k_up[wave] = (int8_t)k_up, info_sh[u & 3].v_up[wave] = (int8_t)v_up;
       k_f = pow2(k_up);
       v_f = pow2(v_up);
     }
@@ -952,8 +979,8 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
         *(u32x4*)(kt + at) = y;
       } else {
         f16x2 h0, l0, h1, l1;
-        split16(__uint_as_float(k_in[j][0]) * k_f, __uint_as_float(k_in[j][1]) * k_f, d.minus1, h0, l0);
-        split16(__uint_as_float(k_in[j][2]) * k_f, __uint_as_float(k_in[j][3]) * k_f, d.minus1, h1, l1);
+        split16(__uint_as_float(k_in[j][0]), __uint_as_float(k_in[j][1]), k_f, d.minus1, h0, l0);
+        split16(__uint_as_float(k_in[j][2]), __uint_as_float(k_in[j][3]), k_f, d.minus1, h1, l1);
         *(f16x4*)(kt + at) = (f16x4){h0[0], h0[1], h1[0], h1[1]};
         *(f16x4*)(kt + T::K_BYTES + at) = (f16x4){l0[0], l0[1], l1[0], l1[1]};
       }
@@ -974,20 +1001,41 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
         *(f16x4*)(vt + at) = (f16x4){(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
       } else {
         f16x2 h0, l0, h1, l1;
-        split16(__uint_as_float(v_in[0][e]) * v_f, __uint_as_float(v_in[1][e]) * v_f, d.minus1, h0, l0);
-        split16(__uint_as_float(v_in[2][e]) * v_f, __uint_as_float(v_in[3][e]) * v_f, d.minus1, h1, l1);
+        split16(__uint_as_float(v_in[0][e]), __uint_as_float(v_in[1][e]), v_f, d.minus1, h0, l0);
+        split16(__uint_as_float(v_in[2][e]), __uint_as_float(v_in[3][e]), v_f, d.minus1, h1, l1);
         *(f16x4*)(vt + at) = (f16x4){h0[0], h0[1], h1[0], h1[1]};
         *(f16x4*)(vt + T::V_BYTES + at) = (f16x4){l0[0], l0[1], l1[0], l1[1]};
       }
     }
   };
-  auto multiply = [&](int u, int k_exp, bool careful) {
+  auto multiply = [&](int u, bool careful) __attribute__((always_inline)) {
     const int base = span.tile(u) * TN, parity = u & 1;
     // Tiles past all of the wave's rows, or before all their windows.
     if (!wave_ok || base > pos_hi || (base + TN - 1 <= below_lo && base >= d.sinks)) return;
-    const bool whole = !__builtin_amdgcn_readfirstlane(hole_sh[u & 3]) && !careful && wave_row + 31 < all_rows && base + TN - 1 <= pos_lo &&
-                       base + TN <= span.end && (base > below_hi || base + TN <= d.sinks);
-    const float back = pow2(-q_up - k_exp);
+    // (Read first and used after the first product, which does not need it.)
+    const u32x4* from = (const u32x4*)&info_sh[u & 3];
+    u32x4 ups = from[0], keys = from[1];
+    bool whole = false;
+    auto look = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        ups[i] = __builtin_amdgcn_readfirstlane(ups[i]), keys[i] = __builtin_amdgcn_readfirstlane(keys[i]);
+      whole = (keys[0] & (TN == 64 ? keys[1] : ~0u)) == ~0u && !careful && wave_row + 31 < all_rows &&
+              base + TN - 1 <= pos_lo && (base > below_hi || base + TN <= d.sinks);
+      if constexpr (SCALED) {
+        int least = 127;
+#pragma unroll
+        for (int i = 0; i < WAVES; i++) least = min(least, (int)(int8_t)(ups[2 + i / 4] >> 8 * (i % 4)));
+        if (least < o_up) {  // larger values than any before: a binade more of room
+          const float f = pow2(least - 1 - o_up);
+          o_up = least - 1;
+#pragma unroll
+          for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[b][e] *= f;
+        }
+      }
+    };
     const char* ks = buffer_sh[parity];
     const char* vs = ks + TERMS * T::K_BYTES;
 #pragma unroll 1
@@ -1008,11 +1056,12 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
             s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.term[0], q_lo[j], s, 0, 0, 0);
             if constexpr (TERMS == 2) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.term[1], q_hi[j], s, 0, 0, 0);
           });
+      if (tb == 0) look();
       if (!whole) {
         // (Without short circuits: a branch for each score costs the registers
         // of several copies of s.)
-        const int in = 32 * tb + 4 * (afresh(lane) >> 5), at = base + in;
-        const uint32_t here = (uint32_t)(seen_sh[u & 3] >> in);
+        const int half = afresh(lane) >> 5, at = base + 32 * tb + 4 * half;
+        const uint32_t here = (tb ? keys[1] : keys[0]) >> 4 * half;
         uint32_t seen = 0;
 #pragma unroll
         for (int e = 0; e < 16; e++) {
@@ -1021,12 +1070,29 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
           s[e] = ok ? s[e] : NEG_INF;
           seen |= (uint32_t)ok << k;
         }
-        if (careful) poison |= (seen & (uint32_t)(bad_sh[u & 3] >> in)) != 0;
+        if (careful) poison |= (seen & (tb ? keys[3] : keys[2]) >> 4 * half) != 0;
       }
-      float top = s[0];
+      // The factors of every 8 keys: of their scores, and of p.  (Values that
+      // are 2^100 below the largest may as well be a little larger; their p
+      // still counts in l.)
+      float back[4];
+      int fall[4];
 #pragma unroll
-      for (int e = 1; e < 16; e++) top = fmaxf(top, s[e]);
-      top = half_max(top) * back;
+      for (int i = 0; i < 4; i++) {
+        back[i] = q_back;
+        fall[i] = 0;
+        if constexpr (SCALED) {
+          const int k_up = (int8_t)((tb ? ups[1] : ups[0]) >> 8 * i);
+          // (Neither 0 nor infinity: a hidden score is -infinity, others may be 0.)
+          back[i] = __builtin_amdgcn_fmed3f(q_back * pow2(-k_up), 1.17549435e-38f, 3.402823466e38f);
+          fall[i] = max(o_up - (int)(int8_t)((tb ? ups[3] : ups[2]) >> 8 * i), -100);
+        }
+      }
+      float top = NEG_INF;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        top = fmaxf(top, fmaxf(fmaxf(s[4 * i], s[4 * i + 1]), fmaxf(s[4 * i + 2], s[4 * i + 3])) * back[i]);
+      top = half_max(top);
       if (__any(top > m + 6.f)) {
         const float m_new = fmaxf(m, top);
         const float fade = __builtin_amdgcn_exp2f(m - (m_new == NEG_INF ? 0.f : m_new));
@@ -1040,18 +1106,22 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
       // p 2^8: at most 2^14.
       const float ref = 8.f - (m == NEG_INF ? 0.f : m);
       f16x8 p_hi[2], p_lo[2];
-      float sum = 0.f;
 #pragma unroll
-      for (int e = 0; e < 16; e += 2) {
-        const float a = __builtin_amdgcn_exp2f(__fmaf_rn(s[e], back, ref));
-        const float b = __builtin_amdgcn_exp2f(__fmaf_rn(s[e + 1], back, ref));
-        sum += a + b;
-        f16x2 hi, lo;
-        split16(a, b, d.minus1, hi, lo);
-        p_hi[e >> 3][e & 7] = hi[0], p_hi[e >> 3][(e & 7) + 1] = hi[1];
-        p_lo[e >> 3][e & 7] = lo[0], p_lo[e >> 3][(e & 7) + 1] = lo[1];
+      for (int i = 0; i < 4; i++) {
+        const float at = ref + (float)fall[i];
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 4 * i; e < 4 * i + 4; e += 2) {
+          const float a = __builtin_amdgcn_exp2f(__fmaf_rn(s[e], back[i], at));
+          const float b = __builtin_amdgcn_exp2f(__fmaf_rn(s[e + 1], back[i], at));
+          sum += a + b;
+          f16x2 hi, lo;
+          split16(a, b, d.minus1, hi, lo);
+          p_hi[e >> 3][e & 7] = hi[0], p_hi[e >> 3][(e & 7) + 1] = hi[1];
+          p_lo[e >> 3][e & 7] = lo[0], p_lo[e >> 3][(e & 7) + 1] = lo[1];
+        }
+        l = SCALED ? __fmaf_rn(sum, pow2(-fall[i]), l) : l + sum;
       }
-      l += sum;
       pipelined<2 * NB, AHEAD, Operands>(
           [&](int i) {
             const int c = i / NB, b = i % NB;
@@ -1070,14 +1140,22 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
     }
   };
   // A tile's buffer, tops and flags go by the parity of its number.
-  auto pass = [&](bool careful) {
+  auto pass = [&](bool careful) __attribute__((always_inline)) {
     m = NEG_INF, l = 0.f;
-    o_up = v_up = 113;  // as for values that are all zero or very small
+    o_up = 113;  // as for values that are all zero or very small
     poison = false;
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
       for (int e = 0; e < 16; e++) o[b][e] = 0.f;
+    auto advance = [&](int u) __attribute__((always_inline)) {
+      if (u + 1 < u1) stage(u + 1, careful);
+      load(u + 2);
+      if (wave == 0) {
+        find_rows(u + 3);
+        find_page(u + 4);
+      }
+    };
     find_page(u0);
     find_rows(u0);
     find_page(u0 + 1);
@@ -1085,32 +1163,17 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
     find_page(u0 + 2);
     __syncthreads();
     load(u0);
-    measure(u0, careful);
     find_rows(u0 + 2);
     find_page(u0 + 3);
-    __syncthreads();
-    stage(u0 & 1);
+    stage(u0, careful);
     load(u0 + 1);
-    measure(u0 + 1, careful);
     for (int u = u0; u < u1; u++) {
-      const int k_exp = k_up, v_exp = v_up;
-      // Tile u is in its buffer, u + 1's tops and u + 2's rows are there, and
-      // nobody reads u - 1 any more.
+      // Tile u is in its buffer, u + 2's rows are there, and nobody reads u - 1
+      // any more.
       __syncthreads();
-      if (u + 1 < u1) stage((u + 1) & 1);
-      load(u + 2);
-      find_rows(u + 3);
-      find_page(u + 4);
-      if (SCALED && v_exp != o_up) {
-        const float f = pow2(v_exp - o_up);
-        o_up = v_exp;
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-          for (int e = 0; e < 16; e++) o[b][e] *= f;
-      }
-      multiply(u, k_exp, careful);
-      measure(u + 2, careful);
+      if (wave < 4) advance(u);
+      multiply(u, careful);
+      if (wave >= 4) advance(u);
     }
     __syncthreads();
   };
