@@ -37,13 +37,15 @@ __device__ __forceinline__ int seq_start(const SeqView& v, int s) {
   return a < 0 ? 0 : a > v.tokens ? v.tokens : a;
 }
 
-// The page of token `tok` of the sequence with page row `row`, or -1 where
-// there is none (past the table, or an entry outside the cache).
-__device__ __forceinline__ int page_of(const int* row, int max_pages, const CacheView& c, int tok) {
+// The entry for token `tok` in the page row `row`, -1 past the table.  What it
+// is is looked at only where it is needed (page_ok): a check right behind the
+// load would wait for it, and for every load before it.
+__device__ __forceinline__ int page_entry(const int* row, int max_pages, const CacheView& c, int tok) {
   const int at = fdiv(tok, c.page_div);
-  if (at >= max_pages) return -1;
-  const int p = row[at];
-  return (unsigned)p < (uint64_t)c.n_pages ? p : -1;
+  return at < max_pages ? row[at] : -1;
+}
+__device__ __forceinline__ bool page_ok(const CacheView& c, int page) {
+  return (unsigned)page < (uint64_t)c.n_pages;
 }
 
 rtenhip_status cache_view(const rtenhip_kv_cache* cache, CacheView& v, int& dtype);

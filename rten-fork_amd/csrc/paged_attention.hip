@@ -317,46 +317,43 @@ struct CacheType {
 //    dimensions, so nothing moves between lanes.
 // An f32 cache uses the f32 instructions, f16 splits q and p into two f16
 // terms (exact products, 22 bits of q and p), bf16 into three bf16 terms.
-// Bound by the cache's bytes: while one tile is worked on, the next tile's
-// keys and this one's values are on their way.
+// Bound by the cache's bytes: DEPTH tiles are on their way in registers while
+// one is worked on.
 template <int DP, int TYPE>
 struct DecodeTile {
   static constexpr int DPL = DP / 16;                                // value dimensions of a lane
   static constexpr int KV = DP * CacheType<TYPE>::size / 64;         // 16-byte loads of keys
   static constexpr int VW = DPL * CacheType<TYPE>::size / 4;         // 32-bit words of values, per key
+  // Tiles in flight, as many as leave two waves to a SIMD (one at DP = 256).
+  static constexpr int DEPTH = DP == 64 ? (TYPE == RTENHIP_CACHE_F32 ? 3 : 4) : 2;
   static constexpr int QW = TYPE == RTENHIP_CACHE_F32 ? DP / 4 : TYPE == RTENHIP_CACHE_F16 ? DP / 4 : 3 * DP / 8;
 };
 
-// (Past head_dim the row's last 16 bytes again: q is zero there, and those
-// results are not stored.)
+// Rows are loaded whether there is a key or not (then the cache's first row,
+// which there always is), and what must not count is cleared when it is used: a
+// load under a condition would be waited for where the paths meet.
+// Past head_dim the row's last 16 bytes are read again: q is zero there, and
+// those results are not stored.
 template <int DP, int TYPE>
-__device__ __forceinline__ void load_keys(const char* base, int64_t row, int g, int dim, u32x4* k) {
+__device__ __forceinline__ void load_keys(const char* row, int g, int dim, u32x4* k) {
   constexpr int KV = DecodeTile<DP, TYPE>::KV, size = CacheType<TYPE>::size, per = 16 / size;
 #pragma unroll
-  for (int j = 0; j < KV; j++) k[j] = (u32x4){0, 0, 0, 0};
-  if (row >= 0) {
-#pragma unroll
-    for (int j = 0; j < KV; j++) k[j] = *(const u32x4*)(base + row + min((4 * j + g) * per, dim - per) * size);
-  }
+  for (int j = 0; j < KV; j++) k[j] = *(const u32x4*)(row + min((4 * j + g) * per, dim - per) * size);
 }
 
-// WORDS words at byte `at` of a row of `bytes` (zero if row < 0), the row's
-// last ones where there are fewer.
+// WORDS words at byte `at` of a row of `bytes`, its last ones where there are
+// fewer.
 template <int WORDS>
-__device__ __forceinline__ void load_words(const char* base, int64_t row, int at, int bytes, uint32_t* v) {
-#pragma unroll
-  for (int c = 0; c < WORDS; c++) v[c] = 0;
-  if (row < 0) return;
-  const char* p = base + row;
+__device__ __forceinline__ void load_words(const char* row, int at, int bytes, uint32_t* v) {
   if constexpr (WORDS == 1) {
-    v[0] = *(const uint32_t*)(p + min(at, bytes - 4));
+    v[0] = *(const uint32_t*)(row + min(at, bytes - 4));
   } else if constexpr (WORDS == 2) {
-    const u32x2 x = *(const u32x2*)(p + min(at, bytes - 8));
+    const u32x2 x = *(const u32x2*)(row + min(at, bytes - 8));
     v[0] = x[0], v[1] = x[1];
   } else {
 #pragma unroll
     for (int c = 0; c < WORDS; c += 4) {
-      const u32x4 x = *(const u32x4*)(p + min(at + 4 * c, bytes - 16));
+      const u32x4 x = *(const u32x4*)(row + min(at + 4 * c, bytes - 16));
 #pragma unroll
       for (int e = 0; e < 4; e++) v[c + e] = x[e];
     }
@@ -383,7 +380,7 @@ __device__ __forceinline__ bool clean(uint32_t& w) {
 template <int DP, int TYPE>
 __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(PagedDesc d) {
   using T = DecodeTile<DP, TYPE>;
-  constexpr int DPL = T::DPL, KV = T::KV, VW = T::VW, size = CacheType<TYPE>::size;
+  constexpr int DPL = T::DPL, KV = T::KV, VW = T::VW, DEPTH = T::DEPTH, size = CacheType<TYPE>::size;
   __shared__ PlanShared plan_sh;
   __shared__ float o_sh[4][PA_SMALL][DP];
   __shared__ float m_sh[4][PA_SMALL], l_sh[4][PA_SMALL];
@@ -464,49 +461,49 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
   const char* vc = d.c.v + (int64_t)w.head * d.c.v_head * size;
 
   // The lane's key (key i of the wave's 16) in tile u: its page, and its rows'
-  // offsets from that, -1 where no row sees the key or it has no page.
+  // offsets from that, and whether some row sees the key and it has a page.
   auto page_at = [&](int u) {
     if (u >= u1) return -1;
     const int key = span.tile(u) * PA_UNIT + 16 * wave + i;
     if (key >= span.end || (key < span.lo && key >= d.sinks)) return -1;
-    return page_of(table, d.s.max_pages, d.c, key);
+    return page_entry(table, d.s.max_pages, d.c, key);
   };
   auto rows_at = [&](int u, int page, int64_t& k_row, int64_t& v_row) {
     const int key = (u < u1 ? span.tile(u) * PA_UNIT : 0) + 16 * wave + i;
     const int64_t slot = key - fdiv(key, d.c.page_div) * d.c.page_size;
-    k_row = page < 0 ? -1 : (page * d.c.k_page + slot * d.c.k_slot) * size;
-    v_row = page < 0 ? -1 : (page * d.c.v_page + slot * d.c.v_slot) * size;
+    const bool ok = page_ok(d.c, page);
+    k_row = ok ? (page * d.c.k_page + slot * d.c.k_slot) * size : 0;
+    v_row = ok ? (page * d.c.v_page + slot * d.c.v_slot) * size : 0;
+    return ok;
   };
 
   float m, l;
   f32x4 o[DPL];
   bool poison;
-  auto pass = [&](bool careful) {
+  auto pass = [&](bool careful) __attribute__((always_inline)) {
     m = NEG_INF, l = 0.f;
     poison = false;
 #pragma unroll
     for (int e = 0; e < DPL; e++) o[e] = (f32x4){0, 0, 0, 0};
-    int page_next = page_at(u0);
-    int64_t k_row, v_row;
-    rows_at(u0, page_next, k_row, v_row);
-    page_next = page_at(u0 + 1);
-    u32x4 k[KV], k_next[KV];
-    load_keys<DP, TYPE>(kc, k_row, g, dim, k);
-    for (int u = u0; u < u1; u++) {
-      // This tile's values, the next one's keys, the one after's pages.
-      bool here[4];
-      uint32_t v[4][VW];
-      const int base = span.tile(u) * PA_UNIT + 16 * wave + 4 * g;
+    // Tile u is loaded into stage (u - u0) % DEPTH; its page was asked for two
+    // loads before.
+    u32x4 k[DEPTH][KV];
+    uint32_t v[DEPTH][4][VW];
+    uint32_t here[DEPTH];  // which of the lane's four values' keys there are
+    int page_next = page_at(u0), page_after = page_at(u0 + 1);
+    auto fetch = [&](int u, int stage) __attribute__((always_inline)) {
+      int64_t k_row, v_row;
+      const bool ok = rows_at(u, page_next, k_row, v_row);
+      page_next = page_after;
+      page_after = page_at(u + 2);
+      load_keys<DP, TYPE>(kc + k_row, g, dim, k[stage]);
+      here[stage] = (uint32_t)(__ballot(ok) >> (4 * g)) & 15;  // (bits 0 .. 15: the 16 keys)
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int64_t row = __shfl((long long)v_row, 4 * g + r);
-        here[r] = row >= 0;
-        load_words<VW>(vc, row, i * DPL * size, dim * size, v[r]);
-      }
-      rows_at(u + 1, page_next, k_row, v_row);
-      load_keys<DP, TYPE>(kc, k_row, g, dim, k_next);
-      page_next = page_at(u + 2);
-
+      for (int r = 0; r < 4; r++)
+        load_words<VW>(vc + __shfl((long long)v_row, 4 * g + r), i * DPL * size, dim * size, v[stage][r]);
+    };
+    auto work = [&](int u, const u32x4* k, uint32_t (*v)[VW], uint32_t here) __attribute__((always_inline)) {
+      const int base = span.tile(u) * PA_UNIT + 16 * wave + 4 * g;
       f32x4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < KV; j++) {
@@ -541,7 +538,7 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         const int at = base + r;
-        seen[r] = here[r] & (at <= pos) & ((at > below) | (at < d.sinks));
+        seen[r] = (here >> r & 1) & (at <= pos) & ((at > below) | (at < d.sinks));
         p[r] = seen[r] ? (s0[r] + s1[r]) * q_back : NEG_INF;
         top = fmaxf(top, p[r]);
       }
@@ -563,6 +560,12 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
       for (int e = 0; e < DPL; e++)
 #pragma unroll
         for (int r = 0; r < 4; r++) o[e][r] *= fade;
+      if (__any(here != 15)) {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int c = 0; c < VW; c++) v[r][c] = here >> r & 1 ? v[r][c] : 0;
+      }
       if (careful) {
         // A value that is not finite must not meet the zero weight of a row
         // that does not see it; the rows that do see it end as NaN.
@@ -619,8 +622,15 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
           }
         }
       }
+    };
 #pragma unroll
-      for (int j = 0; j < KV; j++) k[j] = k_next[j];
+    for (int s = 0; s < DEPTH; s++) fetch(u0 + s, s);
+    for (int u = u0; u < u1; u += DEPTH) {
+#pragma unroll
+      for (int s = 0; s < DEPTH; s++) {
+        if (u + s < u1) work(u + s, k[s], v[s], here[s]);
+        fetch(u + s + DEPTH, s);
+      }
     }
     l = quarter_sum(l);
   };
@@ -880,44 +890,38 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
           v_key(t >> 5 << 2) {}
   };
   // The rows of a tile: thread i < TN finds key i's page two tiles before the
-  // loads need it and leaves its rows' offsets in LDS; -1 where nobody sees the
-  // key or it has no page.
+  // loads need it and leaves its rows' offsets in LDS, the first row's where
+  // nobody sees the key or it has no page.
   int page_next = -1;
   auto find_page = [&](int u) __attribute__((always_inline)) {
     page_next = -1;
     if (tid >= TN || u >= u1) return;
     const int key = span.tile(u) * TN + tid;
-    if (key < span.end && (key >= span.lo || key < d.sinks)) page_next = page_of(table, d.s.max_pages, d.c, key);
+    if (key < span.end && (key >= span.lo || key < d.sinks)) page_next = page_entry(table, d.s.max_pages, d.c, key);
   };
   auto find_rows = [&](int u) __attribute__((always_inline)) {
     if (tid >= 64) return;
     const int key = (u < u1 ? span.tile(u) * TN : 0) + tid;
-    const bool here = page_next >= 0;
+    const bool here = page_ok(d.c, page_next);
     const uint64_t all = __ballot(here);
     if (tid == 0) info_sh[u & 3].seen = all, info_sh[u & 3].bad = 0;
     if (tid >= TN) return;
     const int64_t slot = key - fdiv(key, d.c.page_div) * d.c.page_size;
-    rows_sh[u & 3][0][tid] = here ? (page_next * d.c.k_page + slot * d.c.k_slot) * size : -1;
-    rows_sh[u & 3][1][tid] = here ? (page_next * d.c.v_page + slot * d.c.v_slot) * size : -1;
+    rows_sh[u & 3][0][tid] = here ? (page_next * d.c.k_page + slot * d.c.k_slot) * size : 0;
+    rows_sh[u & 3][1][tid] = here ? (page_next * d.c.v_page + slot * d.c.v_slot) * size : 0;
   };
   u32x4 k_in[KL];
   uint32_t v_in[4][VW];
-  // (Past head_dim the row's last 16 bytes again: q is zero there, and those
-  // results are not stored.)
   auto load = [&](int u) __attribute__((always_inline)) {
     const Place at(afresh(tid));
-    const int64_t kr = rows_sh[u & 3][0][at.k_row];
+    const char* kr = kc + rows_sh[u & 3][0][at.k_row];
 #pragma unroll
-    for (int j = 0; j < KL; j++) k_in[j] = (u32x4){0, 0, 0, 0};
-    if (kr >= 0) {
-#pragma unroll
-      for (int j = 0; j < KL; j++)
-        k_in[j] = *(const u32x4*)(kc + kr + min((8 * j + at.k_eighth) * PER, dim - PER) * size);
-    }
+    for (int j = 0; j < KL; j++) k_in[j] = *(const u32x4*)(kr + min((8 * j + at.k_eighth) * PER, dim - PER) * size);
 #pragma unroll
     for (int r = 0; r < 4; r++)
-      load_words<VW>(vc, rows_sh[u & 3][1][at.v_key + r], at.v_group * DPV * size, dim * size, v_in[r]);
+      load_words<VW>(vc + rows_sh[u & 3][1][at.v_key + r], at.v_group * DPV * size, dim * size, v_in[r]);
   };
+
   float m, l;
   f32x16 o[NB];
   int o_up;  // o is 2^o_up times the result
@@ -925,6 +929,24 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
   // Converts the tile in the registers into its buffer.
   auto stage = [&](int u, bool careful) __attribute__((always_inline)) {
     const int parity = u & 1;
+    // Rows of keys that nobody sees.
+    const uint64_t seen = info_sh[u & 3].seen;
+    const uint32_t seen_lo = __builtin_amdgcn_readfirstlane((uint32_t)seen);
+    const uint32_t seen_hi = __builtin_amdgcn_readfirstlane((uint32_t)(seen >> 32));
+    if ((seen_lo & (TN == 64 ? seen_hi : ~0u)) != ~0u) {
+      const Place p(afresh(tid));
+      const bool k_here = seen >> p.k_row & 1;
+#pragma unroll
+      for (int j = 0; j < KL; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) k_in[j][e] = k_here ? k_in[j][e] : 0;
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const bool v_here = seen >> (p.v_key + r) & 1;
+#pragma unroll
+        for (int c = 0; c < VW; c++) v_in[r][c] = v_here ? v_in[r][c] : 0;
+      }
+    }
     if (careful) {
 #pragma unroll
       for (int r = 0; r < 4; r++) {
@@ -1150,11 +1172,11 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
       for (int e = 0; e < 16; e++) o[b][e] = 0.f;
     auto advance = [&](int u) __attribute__((always_inline)) {
       if (u + 1 < u1) stage(u + 1, careful);
-      load(u + 2);
       if (wave == 0) {
         find_rows(u + 3);
         find_page(u + 4);
       }
+      load(u + 2);
     };
     find_page(u0);
     find_rows(u0);
@@ -1405,6 +1427,10 @@ extern "C" rtenhip_status rtenhip_paged_attention_f32(rtenhip_ctx* ctx, const rt
   if (!ctx) return fail(RTENHIP_MISSING_INPUTS, "Missing context");
   if (!p.grid_small && !p.grid_big) return RTENHIP_OK;
   d.q = q->data, d.q_t = q->strides[0], d.q_h = q->strides[1];
+  if (d.c.n_pages == 0) {  // nothing to see, but a row to load: any of q's
+    d.c.k = d.c.v = (char*)q->data;
+    d.c.k_head = d.c.v_head = 0;
+  }
   d.out = out->data, d.o_t = out->strides[0], d.o_h = out->strides[1];
   d.window = window;
   d.sinks = window ? sinks : 0;

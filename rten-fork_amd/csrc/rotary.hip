@@ -231,7 +231,7 @@ __global__ __launch_bounds__(ROT_THREADS) void rotary_kernel(RotaryDesc d) {
     const int end = d.s.q_starts ? d.s.q_starts[s + 1] : t + 1;
     pos = d.s.kv_lens[s] - (end - t);
     if (pos >= 0) {
-      page = page_of(d.s.table + (int64_t)s * d.s.table_stride, d.s.max_pages, d.c, pos);
+      page = page_entry(d.s.table + (int64_t)s * d.s.table_stride, d.s.max_pages, d.c, pos);
       slot = pos - fdiv(pos, d.c.page_div) * d.c.page_size;
     }
   }
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(ROT_THREADS) void rotary_kernel(RotaryDesc d) {
         float* p = r < d.hq ? d.qo + t * d.qo_t + r * d.qo_h : d.ko + t * d.ko_t + (r - d.hq) * d.ko_h;
         *(float4*)(p + o0) = make_float4(y[0], y[1], y[2], y[3]);
         *(float4*)(p + o1) = make_float4(y[4], y[5], y[6], y[7]);
-      } else if (page >= 0) {
+      } else if (page_ok(d.c, page)) {
         constexpr int size = TYPE == RTENHIP_CACHE_F32 ? 4 : 2;
         char* row = is_v ? d.c.v + (page * d.c.v_page + slot * d.c.v_slot + (r - d.hq - d.hk) * d.c.v_head) * size
                          : d.c.k + (page * d.c.k_page + slot * d.c.k_slot + (r - d.hq) * d.c.k_head) * size;
