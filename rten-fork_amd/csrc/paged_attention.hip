@@ -145,6 +145,12 @@ __device__ __forceinline__ int wave_scan(int x) {  // inclusive
   return x;
 }
 
+// The stretches that a tile of rows over `units` tiles of keys is cut into:
+// its share of the target, to the nearest.
+__device__ __forceinline__ int parts_of(int units, float ratio) {
+  return max(1, min(units, (int)__fmaf_rn((float)units, ratio, 0.5f)));
+}
+
 // The piece of work of workgroup `block`: false if there is none.  Every
 // workgroup counts for itself (thread i the sequences i * each ..), which
 // costs no launch and no order between workgroups.
@@ -167,15 +173,11 @@ __device__ bool plan(const PagedDesc& d, int block, PlanShared& sh, Work& out) {
   int64_t total = 0;
 #pragma unroll
   for (int i = 0; i < THREADS / 64; i++) total += sh.units[i] * heads;
-  const int64_t target = BIG ? d.target_big : d.target_small;
-  // Keys of a stretch, in tiles: stretches for the whole card, none shorter
-  // than a tile.
-  const int64_t len64 = (total + target - 1) / target;
-  const int len = (int)(len64 < 1 ? 1 : len64 > (1 << 26) ? (1 << 26) : len64);
+  const float ratio = (float)(BIG ? d.target_big : d.target_small) / (float)total;
   int items = 0, slots = 0;
   for (int s = s0; s < s1; s++) {
     const SeqWork w = seq_work<BIG, ROWS>(d, s);
-    const int parts = (w.units + len - 1) / len;
+    const int parts = parts_of(w.units, ratio);
     const int n = w.tiles * heads * parts;
     items += n;
     slots += parts > 1 ? n : 0;
@@ -194,7 +196,7 @@ __device__ bool plan(const PagedDesc& d, int block, PlanShared& sh, Work& out) {
   if (block >= at && block < at + items) {
     for (int s = s0; s < s1; s++) {
       const SeqWork w = seq_work<BIG, ROWS>(d, s);
-      const int parts = (w.units + len - 1) / len;
+      const int parts = parts_of(w.units, ratio);
       const int n = w.tiles * heads * parts;
       if (block < at + n) {
         int i = block - at;
@@ -324,8 +326,12 @@ struct DecodeTile {
   static constexpr int DPL = DP / 16;                                // value dimensions of a lane
   static constexpr int KV = DP * CacheType<TYPE>::size / 64;         // 16-byte loads of keys
   static constexpr int VW = DPL * CacheType<TYPE>::size / 4;         // 32-bit words of values, per key
-  // Tiles in flight, as many as leave two waves to a SIMD (one at DP = 256).
-  static constexpr int DEPTH = DP == 64 ? (TYPE == RTENHIP_CACHE_F32 ? 3 : 4) : 2;
+  // Waves on a SIMD, and tiles in flight in each.  (Two tiles in flight against
+  // one on 64 sequences of up to 6000 keys, f16, head_dim 128: 177 against 182
+  // us; of f32 rows, twice as long, one is enough: 188 against 208 us over
+  // 131,072 keys, where two leave no registers.)
+  static constexpr int WAVES = DP == 64 ? 3 : DP == 128 ? 2 : 1;
+  static constexpr int DEPTH = DP == 64 || (DP == 128 && TYPE != RTENHIP_CACHE_F32) ? 2 : 1;
   static constexpr int QW = TYPE == RTENHIP_CACHE_F32 ? DP / 4 : TYPE == RTENHIP_CACHE_F16 ? DP / 4 : 3 * DP / 8;
 };
 
@@ -335,25 +341,25 @@ struct DecodeTile {
 // Past head_dim the row's last 16 bytes are read again: q is zero there, and
 // those results are not stored.
 template <int DP, int TYPE>
-__device__ __forceinline__ void load_keys(const char* row, int g, int dim, u32x4* k) {
+__device__ __forceinline__ void load_keys(const char* base, uint32_t row, int g, int dim, u32x4* k) {
   constexpr int KV = DecodeTile<DP, TYPE>::KV, size = CacheType<TYPE>::size, per = 16 / size;
 #pragma unroll
-  for (int j = 0; j < KV; j++) k[j] = *(const u32x4*)(row + min((4 * j + g) * per, dim - per) * size);
+  for (int j = 0; j < KV; j++) k[j] = *(const u32x4*)(base + (row + (uint32_t)(min((4 * j + g) * per, dim - per) * size)));
 }
 
-// WORDS words at byte `at` of a row of `bytes`, its last ones where there are
-// fewer.
+// WORDS words at byte `at` of a row of `bytes` bytes, its last ones where there
+// are fewer.
 template <int WORDS>
-__device__ __forceinline__ void load_words(const char* row, int at, int bytes, uint32_t* v) {
+__device__ __forceinline__ void load_words(const char* base, uint32_t row, int at, int bytes, uint32_t* v) {
   if constexpr (WORDS == 1) {
-    v[0] = *(const uint32_t*)(row + min(at, bytes - 4));
+    v[0] = *(const uint32_t*)(base + (row + (uint32_t)min(at, bytes - 4)));
   } else if constexpr (WORDS == 2) {
-    const u32x2 x = *(const u32x2*)(row + min(at, bytes - 8));
+    const u32x2 x = *(const u32x2*)(base + (row + (uint32_t)min(at, bytes - 8)));
     v[0] = x[0], v[1] = x[1];
   } else {
 #pragma unroll
     for (int c = 0; c < WORDS; c += 4) {
-      const u32x4 x = *(const u32x4*)(row + min(at + 4 * c, bytes - 16));
+      const u32x4 x = *(const u32x4*)(base + (row + (uint32_t)min(at + 4 * c, bytes - 16)));
 #pragma unroll
       for (int e = 0; e < 4; e++) v[c + e] = x[e];
     }
@@ -377,8 +383,12 @@ __device__ __forceinline__ bool clean(uint32_t& w) {
   }
 }
 
-template <int DP, int TYPE>
-__global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(PagedDesc d) {
+// ALIGNED: no page ends inside a wave's 16 keys (decode_aligned), so they have
+// one page and their rows' distances fit 32 bits: the addresses are scalars and
+// a register that stays.  Otherwise each lane finds its key's rows and the
+// values' come from the lanes that have them.
+template <int DP, int TYPE, bool ALIGNED>
+__global__ __launch_bounds__(PA_THREADS, (DecodeTile<DP, TYPE>::WAVES)) void decode_kernel(PagedDesc d) {
   using T = DecodeTile<DP, TYPE>;
   constexpr int DPL = T::DPL, KV = T::KV, VW = T::VW, DEPTH = T::DEPTH, size = CacheType<TYPE>::size;
   __shared__ PlanShared plan_sh;
@@ -460,22 +470,17 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
   const char* kc = d.c.k + (int64_t)w.head * d.c.k_head * size;
   const char* vc = d.c.v + (int64_t)w.head * d.c.v_head * size;
 
-  // The lane's key (key i of the wave's 16) in tile u: its page, and its rows'
-  // offsets from that, and whether some row sees the key and it has a page.
+  const int pos_first = w.kv_len - w.q_len, below_last = sinks_only(d, w.kv_len - 1);
+
+  // Key 0 of the wave's 16 in tile u, and whether some row sees a key.
+  auto key_of = [&](int u) { return span.tile(min(u, u1 - 1)) * PA_UNIT + 16 * wave; };
+  auto seen_key = [&](int key) { return (key < span.end) & ((key >= span.lo) | (key < d.sinks)); };
   auto page_at = [&](int u) {
-    if (u >= u1) return -1;
-    const int key = span.tile(u) * PA_UNIT + 16 * wave + i;
-    if (key >= span.end || (key < span.lo && key >= d.sinks)) return -1;
-    return page_entry(table, d.s.max_pages, d.c, key);
+    const int key = key_of(u) + (ALIGNED ? 0 : i);
+    return u < u1 && key < span.end ? page_entry(table, d.s.max_pages, d.c, key) : -1;
   };
-  auto rows_at = [&](int u, int page, int64_t& k_row, int64_t& v_row) {
-    const int key = (u < u1 ? span.tile(u) * PA_UNIT : 0) + 16 * wave + i;
-    const int64_t slot = key - fdiv(key, d.c.page_div) * d.c.page_size;
-    const bool ok = page_ok(d.c, page);
-    k_row = ok ? (page * d.c.k_page + slot * d.c.k_slot) * size : 0;
-    v_row = ok ? (page * d.c.v_page + slot * d.c.v_slot) * size : 0;
-    return ok;
-  };
+  const uint32_t k_lane = ALIGNED ? (uint32_t)(i * d.c.k_slot * size) : 0;
+  const uint32_t v_lane = ALIGNED ? (uint32_t)(4 * g * d.c.v_slot * size) : 0;
 
   float m, l;
   f32x4 o[DPL];
@@ -489,21 +494,35 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
     // loads before.
     u32x4 k[DEPTH][KV];
     uint32_t v[DEPTH][4][VW];
-    uint32_t here[DEPTH];  // which of the lane's four values' keys there are
+    uint32_t here[DEPTH];  // the wave's keys that there are, the lane's four from bit 4 g on
     int page_next = page_at(u0), page_after = page_at(u0 + 1);
     auto fetch = [&](int u, int stage) __attribute__((always_inline)) {
-      int64_t k_row, v_row;
-      const bool ok = rows_at(u, page_next, k_row, v_row);
+      const int page = ALIGNED ? __builtin_amdgcn_readfirstlane(page_next) : page_next;
+      const int key = key_of(u) + (ALIGNED ? 0 : i);
       page_next = page_after;
       page_after = page_at(u + 2);
-      load_keys<DP, TYPE>(kc + k_row, g, dim, k[stage]);
-      here[stage] = (uint32_t)(__ballot(ok) >> (4 * g)) & 15;  // (bits 0 .. 15: the 16 keys)
+      const bool ok = page_ok(d.c, page);
+      const int64_t slot = key - fdiv(key, d.c.page_div) * d.c.page_size;
+      const int64_t k_row = ok ? (page * d.c.k_page + slot * d.c.k_slot) * size : 0;
+      const int64_t v_row = ok ? (page * d.c.v_page + slot * d.c.v_slot) * size : 0;
+      load_keys<DP, TYPE>(kc + k_row, k_lane, g, dim, k[stage]);
+      if constexpr (ALIGNED) {
+        here[stage] = ok ? 0xffff : 0;
 #pragma unroll
-      for (int r = 0; r < 4; r++)
-        load_words<VW>(vc + __shfl((long long)v_row, 4 * g + r), i * DPL * size, dim * size, v[stage][r]);
+        for (int r = 0; r < 4; r++)
+          load_words<VW>(vc + v_row + r * d.c.v_slot * size, v_lane, i * DPL * size, dim * size, v[stage][r]);
+      } else {
+        here[stage] = (uint32_t)__ballot(ok) & 0xffff;
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          load_words<VW>(vc + __shfl((long long)v_row, 4 * g + r), 0, i * DPL * size, dim * size, v[stage][r]);
+      }
     };
     auto work = [&](int u, const u32x4* k, uint32_t (*v)[VW], uint32_t here) __attribute__((always_inline)) {
-      const int base = span.tile(u) * PA_UNIT + 16 * wave + 4 * g;
+      const int key = key_of(u), base = key + 4 * g;
+      // All 16 keys are seen by all rows; by some row.
+      const bool some = here == 0xffff && key + 15 < span.end && (key >= span.lo || key + 15 < d.sinks);
+      const bool all = some && key + 15 <= pos_first && (key > below_last || key + 15 < d.sinks);
       f32x4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < KV; j++) {
@@ -533,19 +552,31 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
           }
         }
       }
-      float p[4], top = NEG_INF;
-      bool seen[4];
+      float p[4];
+      uint32_t seen = 15;  // the lane's keys that its row sees
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int at = base + r;
-        seen[r] = (here >> r & 1) & (at <= pos) & ((at > below) | (at < d.sinks));
-        p[r] = seen[r] ? (s0[r] + s1[r]) * q_back : NEG_INF;
-        top = fmaxf(top, p[r]);
+      for (int r = 0; r < 4; r++) p[r] = (s0[r] + s1[r]) * q_back;
+      if (!all) {
+        seen = 0;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int at = base + r;
+          const bool ok = (here >> (4 * g + r) & 1) & seen_key(at) & (at <= pos) & ((at > below) | (at < d.sinks));
+          seen |= (uint32_t)ok << r;
+          p[r] = ok ? p[r] : NEG_INF;
+        }
       }
-      const float m_new = fmaxf(m, quarter_max(top));
+      const float m_new = fmaxf(m, quarter_max(fmaxf(fmaxf(p[0], p[1]), fmaxf(p[2], p[3]))));
       const float ref = m_new == NEG_INF ? 0.f : m_new;
-      const float fade = __builtin_amdgcn_exp2f(m - ref);
-      m = m_new;
+      if (__any(m_new > m)) {
+        const float fade = __builtin_amdgcn_exp2f(m - ref);
+        m = m_new;
+        l *= fade;
+#pragma unroll
+        for (int e = 0; e < DPL; e++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) o[e][r] *= fade;
+      }
       // f16 terms of p have the most bits where the largest p is 2^14; the
       // factor is in l too.
       constexpr float UP = TYPE == RTENHIP_CACHE_F16 ? 14.f : 0.f;
@@ -555,16 +586,14 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
         p[r] = __builtin_amdgcn_exp2f((p[r] - ref) + UP);
         sum += p[r];
       }
-      l = __fmaf_rn(l, fade, sum);
+      l += sum;
+      if (!some) {
 #pragma unroll
-      for (int e = 0; e < DPL; e++)
+        for (int r = 0; r < 4; r++) {
+          const bool ok = (here >> (4 * g + r) & 1) & seen_key(base + r);
 #pragma unroll
-        for (int r = 0; r < 4; r++) o[e][r] *= fade;
-      if (__any(here != 15)) {
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-#pragma unroll
-          for (int c = 0; c < VW; c++) v[r][c] = here >> r & 1 ? v[r][c] : 0;
+          for (int c = 0; c < VW; c++) v[r][c] = ok ? v[r][c] : 0;
+        }
       }
       if (careful) {
         // A value that is not finite must not meet the zero weight of a row
@@ -575,7 +604,7 @@ __global__ __launch_bounds__(PA_THREADS, DP == 256 ? 1 : 2) void decode_kernel(P
 #pragma unroll
           for (int c = 0; c < VW; c++) bad |= clean<TYPE>(v[r][c]);
           const bool key_bad = (__ballot(bad) >> (16 * g)) & 0xffff;
-          poison |= key_bad && seen[r];
+          poison |= key_bad & (seen >> r & 1);
         }
       }
       if constexpr (TYPE == RTENHIP_CACHE_F32) {
@@ -919,7 +948,7 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
     for (int j = 0; j < KL; j++) k_in[j] = *(const u32x4*)(kr + min((8 * j + at.k_eighth) * PER, dim - PER) * size);
 #pragma unroll
     for (int r = 0; r < 4; r++)
-      load_words<VW>(vc + rows_sh[u & 3][1][at.v_key + r], at.v_group * DPV * size, dim * size, v_in[r]);
+      load_words<VW>(vc + rows_sh[u & 3][1][at.v_key + r], 0, at.v_group * DPV * size, dim * size, v_in[r]);
   };
 
   float m, l;
@@ -1306,11 +1335,24 @@ __global__ __launch_bounds__(PA_THREADS) void merge_kernel(PagedDesc d) {
 
 // ---- host ----------------------------------------------------------------------------
 
-constexpr int PA_TARGET_SMALL = 1024, PA_TARGET_BIG = 512;
+// Stretches that the decode kernel aims for, of which the card's 256 CUs hold
+// `resident` workgroups: as many where the tiles are few, so that all run at
+// once and end together; twice as many where there are many tiles, of lengths
+// that differ, so that they even out (64 ragged sequences: 173 against 186 us).
+// The chunk kernel, one workgroup to a CU, aims for one each: its stretches'
+// results are large, and joining twice as many costs more than they even out
+// (prompts and answers mixed: 145 against 177 us).
+static int decode_target(int resident, int64_t tiles) { return tiles * 2 <= resident ? resident : 2 * resident; }
+constexpr int PA_TARGET_BIG = 256;
 
-// Grids and workspace, from sizes the host knows.  tiles_s heads parts_s summed
-// over the sequences is at most target + the tiles, and a sequence with two
-// stretches or more has less than twice its share of the target.
+template <int DP>
+constexpr int decode_waves() {
+  return DecodeTile<DP, RTENHIP_CACHE_F32>::WAVES;
+}
+
+// Grids and workspace, from sizes the host knows.  A tile has its share of the
+// target rounded, or one stretch: at most target + tiles in all, and where it
+// has two or more at most 4 / 3 of its share.
 struct PagedPlan {
   int64_t grid_small, grid_big, slots_small, slots_big;
   size_t bytes;
@@ -1346,13 +1388,16 @@ static rtenhip_status paged_plan(const rtenhip_tensor* q, const rtenhip_kv_cache
   if (tokens && n) {
     const int64_t small_tiles = std::min(n, tokens) * hk;
     const int64_t big_tiles = (tokens * group / d.rows_big + std::min(n, tokens)) * hk;
-    if (small) p.grid_small = small_tiles + (splits ? PA_TARGET_SMALL : 0);
-    if (big) p.grid_big = big_tiles + (splits ? PA_TARGET_BIG : 0);
+    d.target_small = decode_target(256 * (dim <= 64 ? decode_waves<64>() : dim <= 128 ? decode_waves<128>() : decode_waves<256>()),
+                                   small_tiles);
+    d.target_big = PA_TARGET_BIG;
+    if (small) p.grid_small = small_tiles + (splits ? d.target_small : 0);
+    if (big) p.grid_big = big_tiles + (splits ? d.target_big : 0);
     if (p.grid_small > INT32_MAX || p.grid_big > INT32_MAX)
       return fail(RTENHIP_UNSUPPORTED_VALUE, "Too many query rows");
     if (splits) {
-      p.slots_small = small ? 2 * PA_TARGET_SMALL : 0;
-      p.slots_big = big ? 2 * PA_TARGET_BIG : 0;
+      p.slots_small = small ? d.target_small * 3 / 2 : 0;
+      p.slots_big = big ? d.target_big * 3 / 2 : 0;
     }
   }
   size_t at = 0;
@@ -1374,10 +1419,20 @@ static rtenhip_status paged_plan(const rtenhip_tensor* q, const rtenhip_kv_cache
   return RTENHIP_OK;
 }
 
+// Whether the 16 keys of a decoding wave lie in one page, at distances that fit
+// 32 bits.  (On 64 sequences of pages of 16: see decode_kernel.)
+static bool decode_aligned(const CacheView& c) {
+  const int64_t most = (int64_t(1) << 31) / 64;
+  return c.page_size % 16 == 0 && c.k_slot < most && c.v_slot < most;
+}
+
 template <int DP, int TYPE>
 static void launch_paged(const PagedDesc& d, hipStream_t s) {
-  if (d.grid_small)
-    hipLaunchKernelGGL((decode_kernel<DP, TYPE>), dim3((unsigned)d.grid_small), dim3(PA_THREADS), 0, s, d);
+  const dim3 grid((unsigned)d.grid_small);
+  if (d.grid_small && decode_aligned(d.c))
+    hipLaunchKernelGGL((decode_kernel<DP, TYPE, true>), grid, dim3(PA_THREADS), 0, s, d);
+  else if (d.grid_small)
+    hipLaunchKernelGGL((decode_kernel<DP, TYPE, false>), grid, dim3(PA_THREADS), 0, s, d);
   if (d.grid_big)
     hipLaunchKernelGGL((chunk_kernel<DP, TYPE>), dim3((unsigned)d.grid_big), dim3(ChunkTile<DP, TYPE>::THREADS), 0, s, d);
 }
@@ -1429,7 +1484,7 @@ extern "C" rtenhip_status rtenhip_paged_attention_f32(rtenhip_ctx* ctx, const rt
   d.q = q->data, d.q_t = q->strides[0], d.q_h = q->strides[1];
   if (d.c.n_pages == 0) {  // nothing to see, but a row to load: any of q's
     d.c.k = d.c.v = (char*)q->data;
-    d.c.k_head = d.c.v_head = 0;
+    d.c.k_head = d.c.v_head = d.c.k_slot = d.c.v_slot = 0;
   }
   d.out = out->data, d.o_t = out->strides[0], d.o_h = out->strides[1];
   d.window = window;
@@ -1438,7 +1493,6 @@ extern "C" rtenhip_status rtenhip_paged_attention_f32(rtenhip_ctx* ctx, const rt
   d.minus1 = -1.f;
   d.grid_small = (int)p.grid_small, d.grid_big = (int)p.grid_big;
   d.slots_small = (int)p.slots_small, d.slots_big = (int)p.slots_big;
-  d.target_small = PA_TARGET_SMALL, d.target_big = PA_TARGET_BIG;
   char* ws = (char*)workspace;
   if (p.bytes) {
     d.slots = (int*)(ws + p.slots);
