@@ -177,6 +177,7 @@ class Context:
         if not torch.cuda.is_available():
             raise RuntimeError("rten_hip needs a HIP GPU; none is visible")
         self.device = device
+        self._raw_stream = None
         self.ptr = lib().rtenhip_create(device)
         if not self.ptr:
             raise RuntimeError(lib().rtenhip_last_error_message().decode())
@@ -189,9 +190,16 @@ class Context:
 
     def sync_stream(self, stream=None):
         torch = _torch()
-        s = stream if stream is not None else torch.cuda.current_stream(self.device)
-        check(lib().rtenhip_set_stream(self.ptr, s.cuda_stream))
-        self.stream = s  # the torch stream the context's work is queued on
+        if stream is None:
+            # (A torch stream object takes longer to make than a launch.)
+            raw = torch._C._cuda_getCurrentRawStream(self.device)
+            if raw != self._raw_stream:
+                stream = torch.cuda.current_stream(self.device)
+        else:
+            raw = stream.cuda_stream
+        check(lib().rtenhip_set_stream(self.ptr, raw))
+        if stream is not None:
+            self._raw_stream, self.stream = raw, stream  # the torch stream the context's work is queued on
 
     def use_stream(self, stream):
         """Run this context's graphs on ``stream`` (a torch.cuda.Stream) and

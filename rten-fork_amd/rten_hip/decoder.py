@@ -92,9 +92,10 @@ def _on_device(t, ctx, dtype, what):
 def _rows(t, ctx, what):
     """rtenhip_tensor of a float32 [tokens, heads, head_dim] tensor."""
     _on_device(t, ctx, _torch().float32, what)
-    if t.dim() != 3:
+    shape = t.shape
+    if len(shape) != 3:
         raise OpError(3, "Expected [tokens, heads, head_dim] inputs")
-    return _ROWS.pack(t.data_ptr(), 3, *t.shape, *t.stride())
+    return _ROWS.pack(t.data_ptr(), 3, *shape, *t.stride())
 
 
 def _vector(t, n, ctx, dtype, what):
@@ -160,7 +161,7 @@ def _context(ctx):
     if ctx is None:
         return default_context(), True
     torch = _torch()
-    return ctx, ctx.stream.cuda_stream == torch.cuda.current_stream(ctx.device).cuda_stream
+    return ctx, ctx._raw_stream == torch._C._cuda_getCurrentRawStream(ctx.device)
 
 
 def _empty(like, shape, dtype, ctx, here):
