@@ -11,6 +11,53 @@
 
 namespace rtenhip {
 
+typedef unsigned long long u64;
+
+// ---- sums over a wave ------------------------------------------------------------------
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp(u64 x) {
+  return (u64)dpp<CTRL, ROWS>((uint32_t)(x >> 32)) << 32 | dpp<CTRL, ROWS>((uint32_t)x);
+}
+// Inclusive prefix over the rows of 16 lanes, the halves and the whole of a wave,
+// all of whose lanes are active: shifts within rows, then the last lanes of rows.
+template <typename T>
+__device__ __forceinline__ T row_scan(T x) {
+  x += dpp<0x111, 0xf>(x);
+  x += dpp<0x112, 0xf>(x);
+  x += dpp<0x114, 0xf>(x);
+  x += dpp<0x118, 0xf>(x);
+  return x;
+}
+template <typename T>
+__device__ __forceinline__ T half_scan(T x) {
+  x = row_scan(x);
+  x += dpp<0x142, 0xa>(x);
+  return x;
+}
+template <typename T>
+__device__ __forceinline__ T wave_scan(T x) {
+  x = half_scan(x);
+  x += dpp<0x143, 0xc>(x);
+  return x;
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t x, int lane) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
+}
+__device__ __forceinline__ u64 lane_of(u64 x, int lane) {
+  return (u64)lane_of((uint32_t)(x >> 32), lane) << 32 | lane_of((uint32_t)x, lane);
+}
+template <typename T>
+__device__ __forceinline__ T wave_sum(T x) {
+  return lane_of(wave_scan(x), 63);
+}
+
+// ---- descriptors -----------------------------------------------------------------------
+
 // A paged cache for the kernels: element strides, any order of page, slot and
 // head, head_dim contiguous elements per row.
 struct CacheView {

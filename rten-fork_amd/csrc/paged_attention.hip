@@ -55,7 +55,6 @@ struct PagedDesc {
   int group, window, sinks;
   float scale_log2e;
   float minus1;  // -1, where the compiler must not know it (see split16)
-  int small_only;  // every sequence has at most PA_SMALL rows
   // Workspace: the stretches of the decode grid, then those of the chunk grid.
   int grid_small, grid_big, slots_small, slots_big;
   int target_small, target_big, rows_big;
@@ -135,16 +134,6 @@ struct PlanShared {
   Work work;
 };
 
-__device__ __forceinline__ int wave_scan(int x) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const int y = __shfl_up(x, m);
-    if (lane >= m) x += y;
-  }
-  return x;
-}
-
 // The stretches that a tile of rows over `units` tiles of keys is cut into:
 // its share of the target, to the nearest.
 __device__ __forceinline__ int parts_of(int units, float ratio) {
@@ -165,8 +154,7 @@ __device__ bool plan(const PagedDesc& d, int block, PlanShared& sh, Work& out) {
     const SeqWork w = seq_work<BIG, ROWS>(d, s);
     units += (int64_t)w.tiles * w.units;
   }
-#pragma unroll
-  for (int m = 32; m; m >>= 1) units += __shfl_xor((long long)units, m);
+  units = (int64_t)wave_sum((u64)units);
   if (lane == 0) sh.units[wave] = units;
   if (tid == 0) sh.work.seq = -1;
   __syncthreads();
@@ -182,13 +170,15 @@ __device__ bool plan(const PagedDesc& d, int block, PlanShared& sh, Work& out) {
     items += n;
     slots += parts > 1 ? n : 0;
   }
-  const int items_in = wave_scan(items), slots_in = wave_scan(slots);
+  const int items_in = (int)wave_scan((uint32_t)items), slots_in = (int)wave_scan((uint32_t)slots);
   if (lane == 63) sh.items[wave] = items_in, sh.slots[wave] = slots_in;
   __syncthreads();
   if (block == 0 && tid == 0 && d.slots) {
-    int n = 0;
-    for (int w = 0; w < THREADS / 64; w++) n += sh.slots[w];
-    d.slots[BIG] = min(n, BIG ? d.slots_big : d.slots_small);
+    int n = 0, all = 0;
+    for (int w = 0; w < THREADS / 64; w++) n += sh.slots[w], all += sh.items[w];
+    // (More pieces than workgroups: q_starts do not rise, and some stretches
+    // never come.  Nothing is joined then.)
+    d.slots[BIG] = all > (int)gridDim.x ? 0 : min(n, BIG ? d.slots_big : d.slots_small);
     if (!(BIG ? d.grid_small : d.grid_big)) d.slots[!BIG] = 0;  // the other kernel does not run
   }
   int at = items_in - items, slot = slots_in - slots;
