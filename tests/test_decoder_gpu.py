@@ -518,8 +518,11 @@ def sample_ref(x, u, t, k, p, mp):
     c = np.cumsum(m[kept])
     at = min(max(u, 0.0), 0.99999994) * c[-1]
     i = int(np.searchsorted(c, at, side="right"))
-    # Weights are whole multiples of 2^-37 or less (of the largest), so a
-    # border moves by at most 2^17 half steps of them.
+    # A border is a share F of the whole.  Weights that are off by up to 2^-31.5
+    # of themselves move it by F (1 - F) 2 2^-31.5 <= 2^-32.5; the rounding to
+    # whole multiples of 2^-46 (50,001 tokens; twice that for up to 131,072) by
+    # half of one for each token on the smaller side, 2^-32 at most: in all
+    # less than 2^-31.2.  This is 2^-30.97.
     near = np.abs(c - at).min() < 2.0 ** -21 * 1e-3 * c[-1]
     return int(kept[i]), math.log(m[kept[i]] / c[-1]), near and at > 0
 
@@ -627,3 +630,250 @@ def test_sample_strided_rows_and_repeats(rh):
     want = [sample_ref(wide[2].copy(), float(v), 1.0, 0, float(np.float32(0.8)), 0.0)[0] for v in u]
     assert e[0].tolist() == want
     assert rh.sample(d[:0], du[:0])[0].shape == (0,)
+
+
+@pytest.mark.parametrize("f", [dict(top_k=129), dict(top_k=5000, top_p=0.9), dict(top_k=3, top_p=0.3), dict(top_p=0.97, min_p=0.001),
+                               dict(min_p=0.05), dict(temperature=30.0, top_p=0.8), dict(temperature=0.01, top_p=0.9),
+                               dict(temperature=30.0, top_k=20000, top_p=0.5, min_p=0.5), dict()], ids=str)
+@pytest.mark.parametrize("vocab", [16384, 16385, 32768, 32769, 131072])
+def test_sample_large_vocabularies(rh, f, vocab):
+    """At the ends of what one workgroup holds and past them: loud, faint,
+    sorted, equal and nearly equal rows."""
+    g = np.random.default_rng(vocab)
+    x = (g.standard_normal((8, vocab)) * 2.5).astype(np.float32)
+    x[1] *= np.float32(0.01)
+    x[2] = np.sort(x[2])
+    x[3] = -np.sort(x[3])
+    x[4] = np.round(x[4])
+    x[5] = np.float32(-1e30)
+    x[6] = np.where(g.random(vocab) < 0.999, np.finfo(np.float32).min, x[6])
+    x[7, g.integers(0, vocab, 3)] = np.inf
+    check_samples(rh, x, g.random(8, dtype=np.float32), **f)
+
+
+# ---------------------------------------------------------------------------
+# Together
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("cache_type,page,window", [("float32", 16, 0), ("float16", 24, 0), ("bfloat16", 8, 40)])
+def test_decoder_run(rh, cache_type, page, window):
+    """Prompts in one step, then token by token, through two layers: every
+    operator against its plain form on what the step gave it, the caches at the
+    end against all tokens' rows."""
+    import copy
+
+    import torch
+
+    prompts, steps, hq, hk, dim, vocab, layers = [70, 5, 33, 1], 5, 4, 2, 64, 1000, 2
+    final = [n + steps for n in prompts]
+    pages = Paged(prompts, final, page, seed=3)
+    g = torch.Generator().manual_seed(11)
+
+    def weights(*shape):
+        return (torch.randn(*shape, generator=g) / math.sqrt(shape[0])).cuda()
+
+    width = hq * dim
+    embedding, head = weights(vocab, width) * math.sqrt(vocab), weights(width, vocab) * 3
+    w_in = [weights(width, (hq + 2 * hk) * dim) for _ in range(layers)]
+    w_out = [weights(width, width) for _ in range(layers)]
+    scales = [(1 + 0.2 * torch.randn(2, dim, generator=g)).cuda() for _ in range(layers)]
+    freq = (10000.0 ** (-torch.arange(dim // 2).double() / (dim // 2))).float().cuda()
+    caches = [[torch.zeros(pages.n_pages, page, hk, dim, dtype=dtype(cache_type)).cuda() for _ in range(2)] for _ in range(layers)]
+    rows = [[[] for _ in prompts] for _ in range(layers)]  # k as it came, of each layer and sequence
+    tokens = torch.randint(0, vocab, (sum(prompts),), generator=g).cuda()
+    f = dict(temperature=0.9, top_k=60, top_p=0.95)
+    for step in range(steps + 1):
+        s = copy.copy(pages)
+        s.q_lens = prompts if step == 0 else [1] * len(prompts)
+        s.kv_lens = [n + step for n in prompts]
+        s.starts = np.concatenate(([0], np.cumsum(s.q_lens)))
+        s.d_kv = torch.tensor(s.kv_lens, dtype=torch.int32).cuda()
+        starts = torch.from_numpy(s.starts.astype(np.int32)).cuda() if step == 0 else None
+        pos = np.concatenate([np.arange(kv - q, kv) for q, kv in zip(s.q_lens, s.kv_lens)])
+        x = embedding[tokens]
+        for i in range(layers):
+            qkv = (x @ w_in[i]).view(-1, hq + 2 * hk, dim)
+            q, k, v = qkv.split([hq, hk, hk], 1)
+            kc, vc = caches[i]
+            turned = rh.qk_norm_rotary_append(q, k, v, freq, kc, vc, s.d_table, s.d_kv, starts, q_scale=scales[i][0],
+                                              k_scale=scales[i][1])
+            rotary_close(turned.cpu().numpy(), rotary_ref(q.cpu().numpy(), pos, freq.cpu().numpy(),
+                                                          scales[i][0].cpu().numpy(), 1e-6, False), "q")
+            o = rh.paged_attention(turned, kc, vc, s.d_table, s.d_kv, starts, window=window, sinks=2 if window else 0)
+            want, tol = attention_ref(turned.cpu().numpy(), kc.cpu().float().numpy(), vc.cpu().float().numpy(), s,
+                                      1 / math.sqrt(dim), window, 2)
+            attention_close(o.cpu().numpy(), want, tol, (step, i))
+            for n in range(len(prompts)):
+                rows[i][n].append(k[int(s.starts[n]):int(s.starts[n + 1])].cpu().numpy())
+            x = x + o.reshape(-1, width) @ w_out[i]
+        logits = x[torch.from_numpy(s.starts[1:] - 1).cuda()] @ head
+        u = np.random.default_rng(step).random(len(prompts), dtype=np.float32)
+        tokens = torch.from_numpy(check_samples(rh, logits.cpu().numpy(), u, **f)).cuda().long()
+    step16 = 0 if cache_type == "float32" else torch.finfo(dtype(cache_type)).eps / 2
+    for i in range(layers):
+        k = caches[i][0].cpu().float().numpy()
+        for n, kv in enumerate(final):
+            want = rotary_ref(np.concatenate(rows[i][n]), np.arange(kv), freq.cpu().numpy(), scales[i][1].cpu().numpy(), 1e-6, False)
+            for j in range(kv):
+                p, o = pages.place(n, j)
+                top = np.abs(want[j]).max(-1, keepdims=True)
+                assert (np.abs(k[p, o] - want[j]) <= 24 * U * top + step16 * (1 + 24 * U) * np.abs(want[j]) + 2.0 ** -25).all()
+
+
+class Step:
+    """One token for each of some sequences: append, attention and a draw, on
+    buffers that stay."""
+
+    def __init__(self, rh, seed, kv_lens, cache_type="float16"):
+        import torch
+
+        self.rh, self.s = rh, Paged([1] * len(kv_lens), [n + 8 for n in kv_lens], 16, seed=seed)
+        g = torch.Generator().manual_seed(seed)
+        n = len(kv_lens)
+        self.kv = torch.tensor(kv_lens, dtype=torch.int32).cuda()
+        self.cache = torch.randn(2, self.s.n_pages, 16, 2, 64, generator=g).to(dtype(cache_type)).cuda()
+        self.qkv, self.logits, self.u = torch.zeros(n, 12, 64).cuda(), torch.zeros(n, 40000).cuda(), torch.zeros(n).cuda()
+        self.freq = torch.ones(32).cuda()
+        self.inputs = [(torch.randn(n, 12, 64, generator=g).cuda(), (torch.randn(n, 40000, generator=g) * 3).cuda(),
+                        torch.rand(n, generator=g).cuda()) for _ in range(5)]
+        self.kv0, self.cache0 = self.kv.clone(), self.cache.clone()
+
+    def reset(self):
+        self.kv.copy_(self.kv0)
+        self.cache.copy_(self.cache0)
+
+    def feed(self, i):
+        for to, x in zip((self.qkv, self.logits, self.u), self.inputs[i]):
+            to.copy_(x)
+        self.kv.add_(1)
+
+    def run(self, ctx=None):
+        q, k, v = self.qkv.split([8, 2, 2], 1)
+        a = (self.cache[0], self.cache[1], self.s.d_table, self.kv)
+        q = self.rh.qk_norm_rotary_append(q, k, v, self.freq, *a, ctx=ctx)
+        o = self.rh.paged_attention(q, *a, ctx=ctx)
+        return (q, o, *self.rh.sample(self.logits, self.u, top_p=0.9, ctx=ctx), *self.rh.sample(self.logits[:, :5000], self.u, top_k=50, ctx=ctx))
+
+    def eager(self):
+        self.reset()
+        want = []
+        for i in range(len(self.inputs)):
+            self.feed(i)
+            want.append([x.clone() for x in self.run()])
+        return want, self.cache.clone()
+
+
+def same(a, b):
+    import torch
+
+    return all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_decoder_step_captured(rh):
+    """A captured step, replayed on changing inputs and lengths with eager work
+    between, gives the eager steps' bits; so do two graphs, replayed in turn on
+    two streams."""
+    import torch
+
+    steps = [Step(rh, 1, [5, 900, 64, 3000]), Step(rh, 2, [17, 2, 40])]
+    wants = [s.eager() for s in steps]
+    graphs, outs = [], []
+    for s in steps:
+        s.reset()
+        s.feed(0)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            s.run()
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(s.run())
+        graphs.append(g)
+    for s, (want, cache), g, out in zip(steps, wants, graphs, outs):
+        s.reset()
+        for i in range(len(want)):
+            s.feed(i)
+            g.replay()
+            assert same(out, want[i]), i
+            rh.sample(s.logits, s.u, top_k=7)  # eager work between
+            torch.cuda.synchronize()
+        assert torch.equal(s.cache, cache)
+    streams = [torch.cuda.Stream() for _ in steps]
+    for s in steps:
+        s.reset()
+    for i in range(len(wants[0][0])):
+        for s in steps:
+            s.feed(i)
+        for g, st in zip(graphs, streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                g.replay()
+        for st in streams:
+            torch.cuda.current_stream().wait_stream(st)
+        for out, (want, _) in zip(outs, wants):
+            assert same(out, want[i]), i
+
+
+def test_decoder_own_context(rh):
+    """A context on a stream of its own, torch's current stream another one;
+    two contexts at once."""
+    import torch
+
+    steps = [Step(rh, 3, [300, 31]), Step(rh, 4, [16, 4000])]
+    wants = [s.eager() for s in steps]
+    ctxs, streams = [rh.Context(0) for _ in steps], [torch.cuda.Stream() for _ in steps]
+    for c, st in zip(ctxs, streams):
+        c.sync_stream(st)
+    for s in steps:
+        s.reset()
+    for i in range(len(wants[0][0])):
+        outs = []
+        for s in steps:
+            s.feed(i)
+        for s, c, st in zip(steps, ctxs, streams):
+            st.wait_stream(torch.cuda.current_stream())
+            outs.append(s.run(c))
+        for st in streams:
+            torch.cuda.current_stream().wait_stream(st)
+        for out, (want, _) in zip(outs, wants):
+            assert same(out, want[i]), i
+    torch.cuda.synchronize()
+    for c in ctxs:
+        c.close()
+
+
+@pytest.mark.parametrize("cache_type", TYPES)
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("q_lens", [[1, 1], [40, 3]])
+def test_decoder_large_cache(rh, cache_type, page, q_lens):
+    """Pages past 2^31 elements and 2^32 bytes of a cache: the bits that a small
+    one gives.  Keys and values lie side by side in one buffer."""
+    import torch
+
+    hk, dim, kv_lens = 8, 128, [200, 90]
+    width = sum(-(-n // page) for n in kv_lens)
+    g = torch.Generator().manual_seed(page)
+    qkv = torch.randn(sum(q_lens), 16 + 2 * hk, dim, generator=g).cuda()
+    start = torch.tensor([0, q_lens[0], sum(q_lens)], dtype=torch.int32).cuda()
+    kv = torch.tensor(kv_lens, dtype=torch.int32).cuda()
+    old = torch.randn(width, 2, page, hk, dim, generator=g).to(dtype(cache_type))
+    got = []
+    for n_pages in (width, 2 ** 31 // (page * hk * dim) + 3 * width):
+        cache = torch.empty(n_pages, 2, page, hk, dim, dtype=dtype(cache_type), device="cuda")
+        cache[n_pages - width:] = old.cuda()
+        table = torch.full((2, width), -1, dtype=torch.int32)
+        at = 0
+        for s, n in enumerate(kv_lens):
+            for p in range(-(-n // page)):
+                table[s, p] = n_pages - 1 - at
+                at += 1
+        q, k, v = qkv.split([16, hk, hk], 1)
+        a = (cache[:, 0], cache[:, 1], table.cuda(), kv, start)
+        q = rh.qk_norm_rotary_append(q, k, v, None, *a)
+        o = rh.paged_attention(q, *a)
+        got.append((q, o, rh.paged_attention(q, *a), cache[n_pages - width:].clone()))
+        del cache, a
+    torch.cuda.empty_cache()
+    assert same(*got) and torch.equal(got[0][1], got[0][2])
+    assert got[0][1].abs().min() > 0
