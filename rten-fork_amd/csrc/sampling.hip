@@ -57,6 +57,23 @@ __host__ __device__ inline Hist hist_at(void* p) {
   return h;
 }
 
+// What the histogram says of a row: tokens of bins below `lo` are kept, those
+// of lo..hi and of the bin `k` in which top-k ends are gathered, the rest is
+// dropped.
+struct Plan {
+  int lo, hi, k;     // k = -1: top-k drops nothing
+  bool p, slow;      // slow: too many to gather
+  uint32_t first_k;  // gathered ones before bin k
+  u64 n_lo, n_k;     // tokens before bins lo and k
+  u64 m_lo, m_k, total;  // weights; total: of all tokens
+};
+
+// The same with the row's extremes, for the draw.
+struct RowPlan {
+  Plan plan;
+  float top, least;
+};
+
 struct SampleDesc {
   const float* logits;
   int64_t row_stride;
@@ -77,6 +94,7 @@ struct SampleDesc {
   char* hist;       // [rows][cuts] of SA_HIST_BYTES
   u64* list;        // [rows][SA_CAP]
   uint32_t* listed;  // [rows]
+  RowPlan* plans;    // [rows]
 };
 
 // A row's random number, brought into [0, 1).
@@ -474,19 +492,9 @@ __device__ __forceinline__ u64 p_target(float p, u64 total) {
   return n < 1 ? 1 : n > total ? total : n;
 }
 
-// What the histogram says of a row: tokens of bins below `lo` are kept, those
-// of lo..hi and of the bin `k` in which top-k ends are gathered, the rest is
-// dropped.
-struct Plan {
-  int lo, hi, k;     // k = -1: top-k drops nothing
-  bool p, slow;      // slow: too many to gather
-  uint32_t first_k;  // gathered ones before bin k
-  u64 n_lo, n_k;     // tokens before bins lo and k
-  u64 m_lo, m_k, total;  // weights; total: of all tokens
-};
 template <typename H>
-__device__ __forceinline__ Plan plan_of(const H& h, const Row& r, const Filters& f) {
-  const bool masses = h.masses, counts = h.counts;
+__device__ __forceinline__ Plan plan_of(const Bins<H>& bins, const Row& r, const Filters& f) {
+  const bool masses = bins.h.masses, counts = bins.h.counts;
   Plan q{};
   q.lo = SA_BINS, q.hi = q.k = -1;
   q.p = f.top_p < 1.f;
@@ -495,7 +503,6 @@ __device__ __forceinline__ Plan plan_of(const H& h, const Row& r, const Filters&
     q.slow = true;
     return q;
   }
-  const Bins<H> bins(h);
   Found a{};
   if (f.top_k > 0) {
     a = bins.find(false, (u64)f.top_k);
@@ -863,7 +870,7 @@ __global__ __launch_bounds__(SA_ROW) void sample_row_kernel(SampleDesc d) {
           h, [](int, u64, uint32_t) {}, [&](int i, u64 m, uint32_t c) { h.mass32[i] = m, h.count32[i] = c; });
       __syncthreads();
     }
-    q = plan_of(OneHist{h, d.counts, d.masses}, r, f);
+    q = plan_of(Bins<OneHist>(OneHist{h, d.counts, d.masses}), r, f);
   }
   if (!q.slow) {
     gather(src, r, q, few[tid >> 6], list, &sh.listed, block_mass);
@@ -966,13 +973,18 @@ __global__ __launch_bounds__(SA_SPREAD) void sample_gather_kernel(SampleDesc d) 
   const Cut c(d);
   const Ahead src = c.stretch(d);
   const Filters f = filters_of(d, c.row);
+  // (Also on its way meanwhile; nothing of it is used where there is none.)
+  const Bins<CutHists> bins(
+      CutHists{d.hist + (size_t)c.row * d.cuts * SA_HIST_BYTES, d.cuts, d.hist && d.counts, d.hist && d.masses});
   fill_powers(powers);
   if (threadIdx.x == 0) listed = 0;
   float top, least;
   row_extremes<SA_SPREAD>(d, c.row, top, least, extremes);
-  if (f.greedy || top == SA_NEG_INF) return;
+  const bool last = f.greedy || top == SA_NEG_INF;
   const Row r(f, top, least, d.shift, powers);
-  const Plan q = plan_of(CutHists{d.hist + (size_t)c.row * d.cuts * SA_HIST_BYTES, d.cuts, d.counts, d.masses}, r, f);
+  const Plan q = last ? Plan{} : plan_of(bins, r, f);
+  if (c.b0 == 0 && threadIdx.x == 0) d.plans[c.row] = RowPlan{q, top, least};
+  if (last) return;
   if (q.slow) return;
   gather(src, r, q, few[threadIdx.x >> 6], list, &listed, d.block_mass + (int64_t)c.row * d.blocks);
   __syncthreads();
@@ -993,8 +1005,10 @@ __global__ __launch_bounds__(SA_ROW) void sample_pick_kernel(SampleDesc d) {
   const Filters f = filters_of(d, row);
   const float u = uniform_of(d, row);
   fill_powers(powers);
-  float top, least;
-  row_extremes<SA_ROW>(d, row, top, least, sh.extremes);
+  const RowPlan known = d.plans[row];
+  const uint32_t n = d.listed[row];
+  const float top = known.top;
+  __syncthreads();
   if (top == SA_NEG_INF) {
     if (tid == 0) no_token(d, row);
     return;
@@ -1008,10 +1022,9 @@ __global__ __launch_bounds__(SA_ROW) void sample_pick_kernel(SampleDesc d) {
     return;
   }
   const bool infinite = top == -SA_NEG_INF;
-  const Row r(f, top, least, d.shift, powers);
-  const Plan q = plan_of(CutHists{d.hist + (size_t)row * d.cuts * SA_HIST_BYTES, d.cuts, d.counts, d.masses}, r, f);
+  const Row r(f, top, known.least, d.shift, powers);
+  const Plan q = known.plan;
   u64* block_mass = d.block_mass + (int64_t)row * d.blocks;
-  const uint32_t n = d.listed[row];
   u64 limit;
   if (q.slow || n > SA_CAP) {
     const Whole src{d.logits + (int64_t)row * d.row_stride, d.vocab, d.blocks};
@@ -1151,6 +1164,7 @@ static size_t sample_layout(SampleDesc& d, char* base) {
   d.hist = take(rows * d.cuts * SA_HIST_BYTES);
   d.list = (u64*)take(rows * SA_CAP * 8);
   d.listed = (uint32_t*)take(rows * 4);
+  d.plans = (RowPlan*)take(rows * sizeof(RowPlan));
   return at;
 }
 
