@@ -844,9 +844,12 @@ __global__ __launch_bounds__(SA_ROW) void sample_row_kernel(SampleDesc d) {
   }
   const Row r(f, top, least, d.shift, powers);
   Plan q;
-  if (f.top_k > 0 && f.top_k <= SA_ROW / 4 && !r.flat()) {
+  if (f.top_k > 0 && f.top_k <= SA_ROW / 16 && !r.flat()) {
     // A few: the threads' largest ones alone have top_k in the bins up to some
-    // one, so all of the top_k are in these bins, and not many more are.
+    // one, so all of the top_k are in these bins, and not many more are.  (For
+    // more than 1 / 16 of the threads too many more are: with 30,522 tokens
+    // top-50 took 12 us by the histogram of all and takes 10.7, top-256 took 16
+    // this way and takes 14.)
     float own = SA_NEG_INF;
 #pragma unroll
     for (int k = 0; k < K; k++)
@@ -1219,12 +1222,17 @@ extern "C" rtenhip_status rtenhip_sample_f32(rtenhip_ctx* ctx, const rtenhip_ten
   hipStream_t s = stream_of(ctx);
   const dim3 grid((unsigned)d.rows * (unsigned)d.cuts), rows((unsigned)d.rows), spread(SA_SPREAD), whole(SA_ROW);
   const bool none = greedy || (!k && !p);
-  const int held = (d.blocks + SA_ROW / 64 - 1) / (SA_ROW / 64);  // blocks to a wave
+  const bool plain = !greedy && none && !sampling->min_ps && !(sampling->min_p > 0.f);
+  // Blocks that each wave of a row's workgroup would hold: one or two are held
+  // (64 rows of 32,768, then of 32,769 by the cut kernels: top-p 21 and 29 us,
+  // top-50 11 and 25), but two not without a filter, where the cut kernels read
+  // once and take two launches (13 and 10 us; one row 12 and 8).
+  const int held = (d.blocks + SA_ROW / 64 - 1) / (SA_ROW / 64);
   if (held == 1) {
     hipLaunchKernelGGL((sample_row_kernel<1>), rows, whole, 0, s, d);
-  } else if (held == 2) {
+  } else if (held == 2 && !plain) {
     hipLaunchKernelGGL((sample_row_kernel<2>), rows, whole, 0, s, d);
-  } else if (none && !sampling->min_ps && !(sampling->min_p > 0.f)) {
+  } else if (plain || greedy) {
     hipLaunchKernelGGL(sample_block_kernel, grid, spread, 0, s, d);
     hipLaunchKernelGGL(sample_draw_kernel, rows, whole, 0, s, d);
   } else {
