@@ -331,25 +331,47 @@ struct DecodeTile {
 // Past head_dim the row's last 16 bytes are read again: q is zero there, and
 // those results are not stored.
 template <int DP, int TYPE>
-__device__ __forceinline__ void load_keys(const char* base, uint32_t row, int g, int dim, u32x4* k) {
+__device__ __forceinline__ void load_keys(const char* row, int g, int dim, u32x4* k) {
   constexpr int KV = DecodeTile<DP, TYPE>::KV, size = CacheType<TYPE>::size, per = 16 / size;
 #pragma unroll
-  for (int j = 0; j < KV; j++) k[j] = *(const u32x4*)(base + (row + (uint32_t)(min((4 * j + g) * per, dim - per) * size)));
+  for (int j = 0; j < KV; j++) k[j] = *(const u32x4*)(row + min((4 * j + g) * per, dim - per) * size);
+}
+
+// The same, and the words of load_words, from a row at a scalar address that all
+// lanes share, with each lane's own offset: nothing is left to add.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t from_here(const char* p) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, -1, 0x00020000);
+}
+template <int WORDS>
+__device__ __forceinline__ void load_words(__amdgpu_buffer_rsrc_t base, const uint32_t* lane, uint32_t row, uint32_t* v) {
+  if constexpr (WORDS == 1) {
+    v[0] = __builtin_amdgcn_raw_buffer_load_b32(base, lane[0], row, 0);
+  } else if constexpr (WORDS == 2) {
+    const auto x = __builtin_amdgcn_raw_buffer_load_b64(base, lane[0], row, 0);
+    v[0] = x[0], v[1] = x[1];
+  } else {
+#pragma unroll
+    for (int c = 0; c < WORDS; c += 4) {
+      const auto x = __builtin_amdgcn_raw_buffer_load_b128(base, lane[c / 4], row, 0);
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[c + e] = x[e];
+    }
+  }
 }
 
 // WORDS words at byte `at` of a row of `bytes` bytes, its last ones where there
 // are fewer.
 template <int WORDS>
-__device__ __forceinline__ void load_words(const char* base, uint32_t row, int at, int bytes, uint32_t* v) {
+__device__ __forceinline__ void load_words(const char* row, int at, int bytes, uint32_t* v) {
   if constexpr (WORDS == 1) {
-    v[0] = *(const uint32_t*)(base + (row + (uint32_t)min(at, bytes - 4)));
+    v[0] = *(const uint32_t*)(row + min(at, bytes - 4));
   } else if constexpr (WORDS == 2) {
-    const u32x2 x = *(const u32x2*)(base + (row + (uint32_t)min(at, bytes - 8)));
+    const u32x2 x = *(const u32x2*)(row + min(at, bytes - 8));
     v[0] = x[0], v[1] = x[1];
   } else {
 #pragma unroll
     for (int c = 0; c < WORDS; c += 4) {
-      const u32x4 x = *(const u32x4*)(base + (row + (uint32_t)min(at + 4 * c, bytes - 16)));
+      const u32x4 x = *(const u32x4*)(row + min(at + 4 * c, bytes - 16));
 #pragma unroll
       for (int e = 0; e < 4; e++) v[c + e] = x[e];
     }
@@ -374,8 +396,8 @@ __device__ __forceinline__ bool clean(uint32_t& w) {
 }
 
 // ALIGNED: no page ends inside a wave's 16 keys (decode_aligned), so they have
-// one page and their rows' distances fit 32 bits: the addresses are scalars and
-// a register that stays.  Otherwise each lane finds its key's rows and the
+// one page and their rows' distances fit 32 bits: a tile's addresses are two
+// scalars, and registers that stay.  Otherwise each lane finds its key's rows and the
 // values' come from the lanes that have them.
 template <int DP, int TYPE, bool ALIGNED>
 __global__ __launch_bounds__(PA_THREADS, (DecodeTile<DP, TYPE>::WAVES)) void decode_kernel(PagedDesc d) {
@@ -465,12 +487,24 @@ __global__ __launch_bounds__(PA_THREADS, (DecodeTile<DP, TYPE>::WAVES)) void dec
   // Key 0 of the wave's 16 in tile u, and whether some row sees a key.
   auto key_of = [&](int u) { return span.tile(min(u, u1 - 1)) * PA_UNIT + 16 * wave; };
   auto seen_key = [&](int key) { return (key < span.end) & ((key >= span.lo) | (key < d.sinks)); };
-  auto page_at = [&](int u) {
-    const int key = key_of(u) + (ALIGNED ? 0 : i);
-    return u < u1 && key < span.end ? page_entry(table, d.s.max_pages, d.c, key) : -1;
+  struct Place {
+    int page, slot;
   };
-  const uint32_t k_lane = ALIGNED ? (uint32_t)(i * d.c.k_slot * size) : 0;
-  const uint32_t v_lane = ALIGNED ? (uint32_t)(4 * g * d.c.v_slot * size) : 0;
+  auto page_at = [&](int u) {
+    const int key = key_of(u) + (ALIGNED ? 0 : i), at = fdiv(key, d.c.page_div);
+    return Place{u < u1 && key < span.end && at < d.s.max_pages ? table[at] : -1, key - at * d.c.page_size};
+  };
+  // ALIGNED: a lane's way from its wave's first row, in bytes.
+  constexpr int VL = VW < 4 ? 1 : VW / 4;
+  uint32_t k_lane[KV], v_lane[VL];
+  if constexpr (ALIGNED) {
+    constexpr int per = 16 / size, last = VW < 4 ? VW * 4 : 16;
+#pragma unroll
+    for (int j = 0; j < KV; j++) k_lane[j] = (uint32_t)(i * d.c.k_slot + min((4 * j + g) * per, dim - per)) * size;
+#pragma unroll
+    for (int c = 0; c < VL; c++)
+      v_lane[c] = (uint32_t)(4 * g * d.c.v_slot * size + min(i * DPL * size + 16 * c, dim * size - last));
+  }
 
   float m, l;
   f32x4 o[DPL];
@@ -485,28 +519,31 @@ __global__ __launch_bounds__(PA_THREADS, (DecodeTile<DP, TYPE>::WAVES)) void dec
     u32x4 k[DEPTH][KV];
     uint32_t v[DEPTH][4][VW];
     uint32_t here[DEPTH];  // the wave's keys that there are, the lane's four from bit 4 g on
-    int page_next = page_at(u0), page_after = page_at(u0 + 1);
+    Place next = page_at(u0), after = page_at(u0 + 1);
     auto fetch = [&](int u, int stage) __attribute__((always_inline)) {
-      const int page = ALIGNED ? __builtin_amdgcn_readfirstlane(page_next) : page_next;
-      const int key = key_of(u) + (ALIGNED ? 0 : i);
-      page_next = page_after;
-      page_after = page_at(u + 2);
+      const int page = ALIGNED ? __builtin_amdgcn_readfirstlane(next.page) : next.page;
       const bool ok = page_ok(d.c, page);
-      const int64_t slot = key - fdiv(key, d.c.page_div) * d.c.page_size;
-      const int64_t k_row = ok ? (page * d.c.k_page + slot * d.c.k_slot) * size : 0;
-      const int64_t v_row = ok ? (page * d.c.v_page + slot * d.c.v_slot) * size : 0;
-      load_keys<DP, TYPE>(kc + k_row, k_lane, g, dim, k[stage]);
       if constexpr (ALIGNED) {
+        const uint32_t p = ok ? page : 0, slot = ok ? next.slot : 0;
+        const uint32_t k_slot = (uint32_t)d.c.k_slot * size, v_slot = (uint32_t)d.c.v_slot * size;
+        const auto kr = from_here(kc + ((uint64_t)p * (uint32_t)(d.c.k_page * size) + slot * k_slot));
+        const auto vr = from_here(vc + ((uint64_t)p * (uint32_t)(d.c.v_page * size) + slot * v_slot));
+#pragma unroll
+        for (int j = 0; j < KV; j++) load_words<4>(kr, &k_lane[j], 0, (uint32_t*)&k[stage][j]);
+#pragma unroll
+        for (int r = 0; r < 4; r++) load_words<VW>(vr, v_lane, r * v_slot, v[stage][r]);
         here[stage] = ok ? 0xffff : 0;
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-          load_words<VW>(vc + v_row + r * d.c.v_slot * size, v_lane, i * DPL * size, dim * size, v[stage][r]);
       } else {
-        here[stage] = (uint32_t)__ballot(ok) & 0xffff;
+        const int64_t k_row = ok ? (page * d.c.k_page + next.slot * d.c.k_slot) * size : 0;
+        const int64_t v_row = ok ? (page * d.c.v_page + next.slot * d.c.v_slot) * size : 0;
+        load_keys<DP, TYPE>(kc + k_row, g, dim, k[stage]);
 #pragma unroll
         for (int r = 0; r < 4; r++)
-          load_words<VW>(vc + __shfl((long long)v_row, 4 * g + r), 0, i * DPL * size, dim * size, v[stage][r]);
+          load_words<VW>(vc + __shfl((long long)v_row, 4 * g + r), i * DPL * size, dim * size, v[stage][r]);
+        here[stage] = (uint32_t)__ballot(ok) & 0xffff;
       }
+      next = after;
+      after = page_at(u + 2);
     };
     auto work = [&](int u, const u32x4* k, uint32_t (*v)[VW], uint32_t here) __attribute__((always_inline)) {
       const int key = key_of(u), base = key + 4 * g;
@@ -570,13 +607,11 @@ __global__ __launch_bounds__(PA_THREADS, (DecodeTile<DP, TYPE>::WAVES)) void dec
       // f16 terms of p have the most bits where the largest p is 2^14; the
       // factor is in l too.
       constexpr float UP = TYPE == RTENHIP_CACHE_F16 ? 14.f : 0.f;
-      float sum = 0.f;
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        p[r] = __builtin_amdgcn_exp2f((p[r] - ref) + UP);
-        sum += p[r];
+        p[r] = __builtin_amdgcn_exp2f(UP == 0.f ? p[r] - ref : (p[r] - ref) + UP);
+        l += p[r];
       }
-      l += sum;
       if (!some) {
 #pragma unroll
         for (int r = 0; r < 4; r++) {
@@ -938,7 +973,7 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
     for (int j = 0; j < KL; j++) k_in[j] = *(const u32x4*)(kr + min((8 * j + at.k_eighth) * PER, dim - PER) * size);
 #pragma unroll
     for (int r = 0; r < 4; r++)
-      load_words<VW>(vc + rows_sh[u & 3][1][at.v_key + r], 0, at.v_group * DPV * size, dim * size, v_in[r]);
+      load_words<VW>(vc + rows_sh[u & 3][1][at.v_key + r], at.v_group * DPV * size, dim * size, v_in[r]);
   };
 
   float m, l;
@@ -1409,17 +1444,17 @@ static rtenhip_status paged_plan(const rtenhip_tensor* q, const rtenhip_kv_cache
   return RTENHIP_OK;
 }
 
-// Whether the 16 keys of a decoding wave lie in one page, at distances that fit
-// 32 bits.  (On 64 sequences of pages of 16: see decode_kernel.)
-static bool decode_aligned(const CacheView& c) {
-  const int64_t most = (int64_t(1) << 31) / 64;
-  return c.page_size % 16 == 0 && c.k_slot < most && c.v_slot < most;
+// Whether the 16 keys of a decoding wave lie in one page, and distances within
+// a page, and from one page to the next, fit 31 and 32 bits.
+static bool decode_aligned(const CacheView& c, int size) {
+  const int64_t in_page = (int64_t(1) << 31) / size / c.page_size, page = (int64_t(1) << 32) / size;
+  return c.page_size % 16 == 0 && c.k_slot < in_page && c.v_slot < in_page && c.k_page < page && c.v_page < page;
 }
 
 template <int DP, int TYPE>
 static void launch_paged(const PagedDesc& d, hipStream_t s) {
   const dim3 grid((unsigned)d.grid_small);
-  if (d.grid_small && decode_aligned(d.c))
+  if (d.grid_small && decode_aligned(d.c, CacheType<TYPE>::size))
     hipLaunchKernelGGL((decode_kernel<DP, TYPE, true>), grid, dim3(PA_THREADS), 0, s, d);
   else if (d.grid_small)
     hipLaunchKernelGGL((decode_kernel<DP, TYPE, false>), grid, dim3(PA_THREADS), 0, s, d);
