@@ -475,7 +475,8 @@ typedef struct {
 /* The sequences of a call.  Sequence s has the new tokens q_starts[s] ..
  * q_starts[s + 1] - 1 of the call's rows (q_starts NULL: row s alone, one row
  * per sequence) and kv_lens[s] cached tokens, its new ones being the last of
- * them: new token i has position kv_lens[s] - (new tokens of s) + i.  Token j
+ * them: new token i has position kv_lens[s] - (new tokens of s) + i (tokens
+ * from 2^31 - 256 on are seen by nobody).  Token j
  * is in slot j % page_size of page page_table[s * table_stride + j /
  * page_size]; an entry outside [0, n_pages), such as -1, is no page: nothing
  * is written to it and its tokens are seen by nobody.  q_starts does not
@@ -561,8 +562,9 @@ typedef struct {
 
 /* One token for each row of logits [rows, vocab] (unit stride along vocab).
  * With l the row, max its largest value and T the temperature, token i weighs
- * m_i = exp((l_i - max) / T) (64 bits).  In the order of falling l, equal
- * ones by rising index:
+ * m_i = exp((l_i - max) / T), formed to 2^-31 of itself and rounded to a whole
+ * multiple of 2^-38 at the most (2^-45 up to 131,072 tokens).  In the order of
+ * falling l, equal ones by rising index:
  *   top-k keeps the first k (k <= 0: all);
  *   top-p then keeps the tokens that the kept mass before them is less than
  *     p * (all kept mass) of, the first one always (p >= 1: all);

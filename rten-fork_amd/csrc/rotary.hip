@@ -318,7 +318,9 @@ static rtenhip_status launch_rotary(const RotaryDesc& d, int64_t tokens, hipStre
   const int rpp = ROT_THREADS / lpr;
   // Few tokens: a workgroup per pass of a token's rows, so that no load waits
   // for another; many tokens fill the card by themselves and then share the
-  // turns among all rows.
+  // turns among all rows.  (32 + 8 heads of 128: one token 3.6 against 5.3 us
+  // with one workgroup, 400 tokens 6.2 and 6.3, 1024 10.7 and 10.3, 8192 79 and
+  // 73.)
   const int passes = (d.rows + rpp - 1) / rpp;
   const dim3 grid((unsigned)tokens, (unsigned)(tokens < 512 ? passes : 1));
   if (lpr == 8)
