@@ -3270,6 +3270,13 @@ rtenhip_status Graph::run(const int32_t* in_ids, const rtenhip_tensor* ins, int 
     RTENHIP_HIP_CHECK(hipEventRecord(ev_in, caller));
     RTENHIP_HIP_CHECK(hipStreamWaitEvent(exec_stream, ev_in, 0));
   }
+  if (plan->gather_flag && plan->gchk[plan->gseq % Plan::kGatherChecks].pending) {
+    // (deferred mode) The ring is full: the slot's run must have finished, and
+    // its flag been read, before this run's finish (the last node of a replay)
+    // overwrites it; its error is kept for synchronize(), not given to this run.
+    const rtenhip_status cs = collect_gather_checks(*plan, true);
+    if (cs) return cs;  // a HIP error only
+  }
   ctx->stream = exec_stream;
   rtenhip_status st = RTENHIP_OK;
   auto run_op = [&](int op) -> rtenhip_status { return exec_op(*plan, op); };
@@ -3535,12 +3542,6 @@ rtenhip_status Graph::run(const int32_t* in_ids, const rtenhip_tensor* ins, int 
     // whatever the run's status; an event marks the copy.
     const int slot = (int)(plan->gseq % Plan::kGatherChecks);
     Plan::GatherCheck& c = plan->gchk[slot];
-    if (c.pending) {
-      // (deferred mode) The ring is full: the slot's run must have finished
-      // before reuse; its error is kept for synchronize(), not given to this run.
-      rtenhip_status cs = collect_gather_checks(*plan, true);
-      if (!st) st = cs;  // a HIP error only
-    }
     if (!c.ev) RTENHIP_HIP_CHECK(hipEventCreateWithFlags(&c.ev, hipEventDisableTiming));
     c.host = plan->gring_host + slot;
     // A replay ran the finish as its last node; an eager run (or a replay
