@@ -1158,6 +1158,9 @@ static rtenhip_status sample_sizes(int64_t rows, int64_t vocab, SampleDesc& d) {
   return RTENHIP_OK;
 }
 
+// Blocks that each wave of a row's workgroup would hold.
+static int held_blocks(const SampleDesc& d) { return (d.blocks + SA_ROW / 64 - 1) / (SA_ROW / 64); }
+
 // Lays the workspace out from `base`; its size, which does not depend on the
 // filters.
 static size_t sample_layout(SampleDesc& d, char* base) {
@@ -1168,16 +1171,18 @@ static size_t sample_layout(SampleDesc& d, char* base) {
     return p;
   };
   const size_t rows = (size_t)d.rows;
-  d.cut_max = (float*)take(rows * d.cuts * 4);
-  d.cut_min = (float*)take(rows * d.cuts * 4);
-  d.cut_arg = (int*)take(rows * d.cuts * 4);
   d.block_mass = (u64*)take(rows * d.blocks * 8);
   d.block_max = (float*)take(rows * d.blocks * 4);
   d.block_arg = (int*)take(rows * d.blocks * 4);
-  d.hist = take(rows * d.cuts * SA_HIST_BYTES);
-  d.list = (u64*)take(rows * SA_CAP * 8);
-  d.listed = (uint32_t*)take(rows * 4);
-  d.plans = (RowPlan*)take(rows * sizeof(RowPlan));
+  if (held_blocks(d) > 2) {
+    d.cut_max = (float*)take(rows * d.cuts * 4);
+    d.cut_min = (float*)take(rows * d.cuts * 4);
+    d.cut_arg = (int*)take(rows * d.cuts * 4);
+    d.hist = take(rows * d.cuts * SA_HIST_BYTES);
+    d.list = (u64*)take(rows * SA_CAP * 8);
+    d.listed = (uint32_t*)take(rows * 4);
+    d.plans = (RowPlan*)take(rows * sizeof(RowPlan));
+  }
   return at;
 }
 
@@ -1233,11 +1238,11 @@ extern "C" rtenhip_status rtenhip_sample_f32(rtenhip_ctx* ctx, const rtenhip_ten
   const dim3 grid((unsigned)d.rows * (unsigned)d.cuts), rows((unsigned)d.rows), spread(SA_SPREAD), whole(SA_ROW);
   const bool none = greedy || (!k && !p);
   const bool plain = !greedy && none && !sampling->min_ps && !(sampling->min_p > 0.f);
-  // Blocks that each wave of a row's workgroup would hold: one or two are held
-  // (64 rows of 32,768, then of 32,769 by the cut kernels: top-p 21 and 29 us,
-  // top-50 11 and 25), but two not without a filter, where the cut kernels read
-  // once and take two launches (13 and 10 us; one row 12 and 8).
-  const int held = (d.blocks + SA_ROW / 64 - 1) / (SA_ROW / 64);
+  // One or two blocks to a wave are held (64 rows of 32,768, then of 32,769 by
+  // the cut kernels: top-p 21 and 29 us, top-50 11 and 25), but two not without
+  // a filter, where the cut kernels read once and take two launches (13 and 10
+  // us; one row 12 and 8).
+  const int held = held_blocks(d);
   if (held == 1) {
     hipLaunchKernelGGL((sample_row_kernel<1>), rows, whole, 0, s, d);
   } else if (held == 2 && !plain) {

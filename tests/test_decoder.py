@@ -246,6 +246,19 @@ def test_sample(d):
         assert st == code and text in msg, (kw, st, msg)
 
 
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (4096, 1000), (100, 32768), (1000, 32769), (2, 131072), (1, 1 << 24)])
+def test_sample_workspace(d, rows, vocab):
+    """16 bytes for each 1024 tokens of a row; from 32,769 tokens on what
+    gathers its candidates too, no more than 27 KB for each row and stretch."""
+    need = C.c_size_t()
+    assert call(d, "rtenhip_sample_workspace", rows, vocab, C.byref(need))[0] == 0
+    blocks = -(-vocab // 1024)
+    small = rows * blocks * 16 + 10 * 256
+    stretches = min(64, -(-blocks // 4), max(1, 1024 // rows))
+    assert need.value <= (small if vocab <= 32768 else small + rows * (stretches * 27000 + 10000))
+    assert need.value >= rows * blocks * 16
+
+
 def test_null_descriptors(d):
     n = C.c_size_t()
     assert call(d, "rtenhip_paged_attention_workspace", None, None, None, C.byref(n))[0] == MISSING
