@@ -16,6 +16,7 @@ the context's stream and can be captured.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 import struct
 
@@ -261,6 +262,14 @@ def paged_attention(q, k_cache, v_cache, page_table, kv_lens, q_starts=None, sca
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _sample_workspace(rows, vocab):
+    """A size that depends on these two numbers alone."""
+    need = C.c_size_t()
+    _call("rtenhip_sample_workspace", rows, vocab, C.byref(need))
+    return need.value
+
+
 def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ctx=None):
     """One token of each row of ``logits [rows, vocab]`` by the random numbers
     ``uniforms [rows]`` in [0, 1); returns (tokens int32 [rows], logprobs
@@ -283,10 +292,9 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ctx
     s = _SAMPLING.pack(1. if t else temperature, 1. if p else top_p, 0. if m else min_p,
                        0 if k else min(max(int(top_k), 0), vocab), t, p, m, k)
     u = _vector(uniforms, rows, ctx, f32, "uniforms")
-    need = C.c_size_t()
-    _call("rtenhip_sample_workspace", rows, vocab, C.byref(need))
+    need = _sample_workspace(rows, vocab)
     tokens, logprobs = _empty(logits, (rows,), i32, ctx, here), _empty(logits, (rows,), f32, ctx, here)
-    ws = _empty(logits, (need.value,), torch.uint8, ctx, here)
+    ws = _empty(logits, (need,), torch.uint8, ctx, here)
     _call("rtenhip_sample_f32", ctx.ptr, _MATRIX.pack(logits.data_ptr(), 2, rows, vocab, *logits.stride()), s, u,
-          ws.data_ptr(), need.value, tokens.data_ptr(), logprobs.data_ptr())
+          ws.data_ptr(), need, tokens.data_ptr(), logprobs.data_ptr())
     return tokens, logprobs
