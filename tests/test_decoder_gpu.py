@@ -877,3 +877,50 @@ def test_decoder_large_cache(rh, cache_type, page, q_lens):
     torch.cuda.empty_cache()
     assert same(*got) and torch.equal(got[0][1], got[0][2])
     assert got[0][1].abs().min() > 0
+
+
+@pytest.mark.parametrize("vocab", [20000, 40000])
+def test_sample_filters_of_each_row_large(rh, vocab):
+    """As test_sample_filters_of_each_row, for rows of several blocks and rows
+    that are cut; then each filter's array alone."""
+    g = np.random.default_rng(vocab)
+    rows = 40
+    x = (g.standard_normal((rows, vocab)) * 2).astype(np.float32)
+    x[3], x[4], x[5, 1:] = -np.inf, 2.5, -np.inf
+    u = g.random(rows, dtype=np.float32)
+    f = dict(temperature=g.choice([0.0, 0.5, 1.0, 1.7, np.nan, -1.0], rows).astype(np.float32),
+             top_k=g.choice([-1, 0, 1, 7, 300, 5000, vocab - 1, vocab, 2 ** 31 - 1], rows).astype(np.int32),
+             top_p=g.choice([-1.0, 0.0, 0.1, 0.6, 0.95, 1.0, 2.0], rows).astype(np.float32),
+             min_p=g.choice([-1.0, 0.0, 0.02, 0.5, 1.0], rows).astype(np.float32))
+    check_samples(rh, x, u, **f)
+    for n, v in f.items():
+        check_samples(rh, x, u, **{n: v})
+
+
+def test_decoder_workspaces_hold_anything(rh, monkeypatch):
+    """Memory that comes back with old contents: the same bits."""
+    import torch
+
+    import rten_hip.decoder as D
+
+    s = Step(rh, 9, [5, 900, 64, 3000])
+    want, _ = s.eager()
+    plain = D._empty
+    for byte in (0xff, 0x7f, 0):
+        def dirty(like, shape, dtype, ctx, here):
+            t = plain(like, shape, dtype, ctx, here)
+            t.view(torch.uint8).fill_(byte)
+            return t
+
+        monkeypatch.setattr(D, "_empty", dirty)
+        s.reset()
+        for i in range(3):
+            s.feed(i)
+            assert same(s.run(), want[i])
+            q = s.qkv[:, :8].repeat(40, 1, 1)  # a chunk of 40 tokens, kept as the first run gives it
+            starts = torch.tensor([0, 40, 80, 120, 160], dtype=torch.int32).cuda()
+            o = rh.paged_attention(q, s.cache[0], s.cache[1], s.s.d_table, s.kv, starts)
+            if byte == 0xff and i == 0:
+                first, start = o.clone(), q.clone()
+            if i == 0:
+                assert torch.equal(q, start) and torch.equal(o, first)
