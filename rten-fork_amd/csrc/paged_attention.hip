@@ -149,9 +149,14 @@ __device__ bool plan(const PagedDesc& d, int block, PlanShared& sh, Work& out) {
   const int each = (d.s.n + THREADS - 1) / THREADS;
   const int s0 = tid * each, s1 = min(d.s.n, s0 + each);
   const int heads = d.c.heads;
+  // (The first one's is kept: mostly there is no other, and its lengths take a
+  // round trip to memory each time.)
+  SeqWork first{};
+  if (s0 < s1) first = seq_work<BIG, ROWS>(d, s0);
+  const auto work_of = [&](int s) { return s == s0 ? first : seq_work<BIG, ROWS>(d, s); };
   int64_t units = 0;
   for (int s = s0; s < s1; s++) {
-    const SeqWork w = seq_work<BIG, ROWS>(d, s);
+    const SeqWork w = work_of(s);
     units += (int64_t)w.tiles * w.units;
   }
   units = (int64_t)wave_sum((u64)units);
@@ -164,7 +169,7 @@ __device__ bool plan(const PagedDesc& d, int block, PlanShared& sh, Work& out) {
   const float ratio = (float)(BIG ? d.target_big : d.target_small) / (float)total;
   int items = 0, slots = 0;
   for (int s = s0; s < s1; s++) {
-    const SeqWork w = seq_work<BIG, ROWS>(d, s);
+    const SeqWork w = work_of(s);
     const int parts = parts_of(w.units, ratio);
     const int n = w.tiles * heads * parts;
     items += n;
@@ -185,7 +190,7 @@ __device__ bool plan(const PagedDesc& d, int block, PlanShared& sh, Work& out) {
   for (int w = 0; w < wave; w++) at += sh.items[w], slot += sh.slots[w];
   if (block >= at && block < at + items) {
     for (int s = s0; s < s1; s++) {
-      const SeqWork w = seq_work<BIG, ROWS>(d, s);
+      const SeqWork w = work_of(s);
       const int parts = parts_of(w.units, ratio);
       const int n = w.tiles * heads * parts;
       if (block < at + n) {
