@@ -574,8 +574,9 @@ typedef struct {
  * of the indices, exceeds u * (all kept mass), u = uniforms[row] in [0, 1)
  * (brought into that range); logprobs[row] (NULL: not wanted) is the log of
  * its share of the kept mass.  T <= 0 or NaN: the largest l, the first of
- * equals, log 0.  NaN counts as -infinity and is never taken; of +infinities
- * each weighs 1 and the rest 0; a row of nothing else gives -1 and -infinity.
+ * equals, log 0; T infinite: every finite l weighs 1.  NaN counts as -infinity;
+ * -infinity weighs 0 and is never taken; of +infinities each weighs 1 and the
+ * rest 0; a row of nothing but -infinity gives -1 and -infinity.
  * vocab from 1 to 2^24.  workspace as for rtenhip_paged_attention_f32. */
 rtenhip_status rtenhip_sample_workspace(int64_t rows, int64_t vocab, size_t* bytes);
 rtenhip_status rtenhip_sample_f32(rtenhip_ctx* ctx, const rtenhip_tensor* logits,

@@ -159,7 +159,10 @@ struct Row {
     const float m = infinite ? 0.f : row_max;
     max = m;
     inv_t = 1. / (double)f.temperature;
-    scale = __builtin_fmax(inv_t * 1.44269504088896340736, 1e-300);
+    // floor * scale is -64 at every temperature, so that what is masked or no
+    // number weighs nothing at an infinite one either, where any other token
+    // weighs 1.
+    scale = __builtin_fmax(inv_t * 1.44269504088896340736, 64e-290);
     floor = -__builtin_fmin(64. * 0.69314718055994530942 * (double)f.temperature, 1e290);
     base = 6144. + shift;
     min_p = ldexp(f.min_p > 1.f ? 1. : f.min_p > 0.f ? (double)f.min_p : 0., shift);

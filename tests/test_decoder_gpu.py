@@ -924,3 +924,37 @@ def test_decoder_workspaces_hold_anything(rh, monkeypatch):
                 first, start = o.clone(), q.clone()
             if i == 0:
                 assert torch.equal(q, start) and torch.equal(o, first)
+
+
+@pytest.mark.parametrize("f", [dict(), dict(top_k=7), dict(top_k=700), dict(top_p=0.4), dict(top_k=300, top_p=0.7),
+                               dict(min_p=0.5), dict(top_p=0.9, min_p=1.0)], ids=str)
+@pytest.mark.parametrize("vocab", [5, 1000, 30522, 40000])
+def test_sample_infinite_temperature(rh, f, vocab):
+    """All finite logits weigh the same; -infinity, NaN and what lies behind
+    the row weigh nothing."""
+    import torch
+
+    g = np.random.default_rng(vocab)
+    rows = 48
+    x = (g.standard_normal((rows, vocab)) * 3).astype(np.float32)
+    x[1::4][g.random((rows // 4, vocab)) < 0.6] = -np.inf
+    x[2::4][g.random((rows // 4, vocab)) < 0.6] = np.nan
+    x[3::4, vocab // 2:] = np.finfo(np.float32).min
+    x[:, 1] = 2.0  # (some token is always there)
+    u = np.linspace(0, 0.999999, rows).astype(np.float32)
+    d, du = torch.from_numpy(x).cuda(), torch.from_numpy(u).cuda()
+    arrays = dict(f, temperature=torch.full((rows,), math.inf).cuda())
+    a, b = rh.sample(d, du, temperature=math.inf, **f), rh.sample(d, du, **arrays)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    tokens, logprobs = a[0].cpu().numpy(), a[1].cpu().numpy()
+    for r in range(rows):
+        y = np.where(np.isnan(x[r]), -np.inf, x[r]).astype(np.float64)
+        order = np.lexsort((np.arange(vocab), -y))[:np.isfinite(y).sum()]
+        order = order[:f.get("top_k", vocab)]
+        # (Counts times a 24-bit number are exact.)
+        n = len(order)
+        order = order[:int((np.arange(n) < float(np.float32(f.get("top_p", 1.0))) * n).sum())]
+        kept = np.sort(order)
+        assert tokens[r] == kept[int(float(u[r]) * len(kept))], (r, tokens[r])
+        want = -math.log(len(kept))
+        assert abs(logprobs[r] - want) <= 2 * U * max(1.0, -want), (r, logprobs[r], want)
