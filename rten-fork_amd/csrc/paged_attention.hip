@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace rtenhip {
 
@@ -243,25 +244,36 @@ template <int CTRL>
 __device__ __forceinline__ uint32_t max_dpp(uint32_t x) {
   return max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xF, 0xF, true));
 }
-// The largest of the wave's numbers, none negative (their bits are in the
-// same order).
-__device__ __forceinline__ float wave_max(float y) {
+// The largest of numbers of which none is negative (their bits are in the same
+// order): over every 8 lanes, and from those over the wave.
+__device__ __forceinline__ uint32_t eighth_max(float y) {
   uint32_t x = __float_as_uint(y);
-  x = max_dpp<0xB1>(x);   // lane ^ 1
-  x = max_dpp<0x4E>(x);   // lane ^ 2
-  x = max_dpp<0x141>(x);  // mirrored in its 8
+  x = max_dpp<0xB1>(x);         // lane ^ 1
+  x = max_dpp<0x4E>(x);         // lane ^ 2
+  return max_dpp<0x141>(x);     // mirrored in its 8
+}
+__device__ __forceinline__ uint32_t wave_max_of_eighths(uint32_t x) {
   x = max_dpp<0x140>(x);  // mirrored in its 16
   const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
   x = max(r[0], r[1]);
   const auto s = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-  return __uint_as_float(max(s[0], s[1]));
+  return max(s[0], s[1]);
 }
+// The smallest, likewise.
+__device__ __forceinline__ uint32_t wave_min_of_eighths(uint32_t x) {
+  x = min(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x140, 0xF, 0xF, true));
+  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = min(r[0], r[1]);
+  const auto s = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return min(s[0], s[1]);
+}
+__device__ __forceinline__ float wave_max(float y) { return __uint_as_float(wave_max_of_eighths(eighth_max(y))); }
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
 // The power of two that brings a largest magnitude `big` to [2^13, 2^14), as
 // an exponent; what is not finite or very small counts as the nearest that is
-// in range, zero as 1.
+// in range, zero as 2^-100.
 __device__ __forceinline__ int exponent_for(float big) {
   int e = (int)((__float_as_uint(big) >> 23) & 255) - 127;
   e = e > 127 ? 127 : e < -100 ? -100 : e;
@@ -759,6 +771,11 @@ __global__ __launch_bounds__(PA_THREADS, (DecodeTile<DP, TYPE>::WAVES)) void dec
 //    2^-38 of it; q has one for each row, p the factor 2^8.  Powers of two come
 //    out again exactly: a score is multiplied by its keys' and its row's on
 //    its way into the exponential, whose argument takes the values'.
+//    Not all rows see all of 8 keys, and a loud one must not cost its
+//    neighbours their bits: where the largest numbers of 8 keys are more than
+//    2^EVEN apart (an infinity always is), the stretch is computed again with a
+//    power of two for each key (careful).  Up to there a key is exact to 2^-26
+//    of its own largest number, which is finer than the split's 22 bits.
 //  - S^T = K Q^T: a lane (n, h) has row n's scores for the keys
 //    8 i + 4 h + j of each 32, so the softmax needs one exchange with lane
 //    ^ 32, and
@@ -845,6 +862,10 @@ struct __attribute__((aligned(16))) TileInfo {
   uint64_t seen, bad;
 };
 
+// How many binades the largest numbers of 8 keys may lie apart to share an
+// exponent.
+constexpr uint32_t EVEN = 12;
+
 // x, of which the compiler does not know that it is the same in every round of
 // a loop: what follows from it is formed again there, a few instructions,
 // instead of being held in a register that the products' operands need.
@@ -885,6 +906,8 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
   // [tile & 3], as they are read late.
   __shared__ int64_t rows_sh[4][2][TN];  // the keys' and the values' rows
   __shared__ TileInfo info_sh[4];
+  __shared__ __attribute__((aligned(4))) int8_t key_up_sh[SCALED ? 4 : 1][TN];  // each key's exponent, with care
+  __shared__ int uneven_sh;
   Work w;
   if (!plan<true, T::THREADS, T::ROWS>(d, blockIdx.x, plan_sh, w) || w.slot >= d.slots_big) return;
   const int row0 = w.tile * T::ROWS;
@@ -994,7 +1017,8 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
   int o_up;  // o is 2^o_up times the result
   bool poison;
   // Converts the tile in the registers into its buffer.
-  auto stage = [&](int u, bool careful) __attribute__((always_inline)) {
+  auto stage = [&](int u, auto with_care) __attribute__((always_inline)) {
+    constexpr bool careful = decltype(with_care)::value;
     const int parity = u & 1;
     // Rows of keys that nobody sees.
     const uint64_t seen = info_sh[u & 3].seen;
@@ -1014,7 +1038,7 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
         for (int c = 0; c < VW; c++) v_in[r][c] = v_here ? v_in[r][c] : 0;
       }
     }
-    if (careful) {
+    if constexpr (careful) {
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         bool bad = false;
@@ -1026,7 +1050,7 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
     float k_f = 1.f, v_f = 1.f;
     if constexpr (SCALED) {
       float k_top = 0.f, v_top = 0.f;
-      if (careful) {
+      if constexpr (careful) {
 #pragma unroll
         for (int j = 0; j < KL; j++)
 #pragma unroll
@@ -1046,10 +1070,24 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
         v_top = top_of<TYPE>(v_top, v_in[0][c], v_in[1][c]);
         v_top = top_of<TYPE>(v_top, v_in[2][c], v_in[3][c]);
       }
-      const int k_up = __builtin_amdgcn_readfirstlane(exponent_for(wave_max(k_top)));
+      const uint32_t own = eighth_max(k_top);  // the lane's key's
+      if constexpr (careful) {
+        const int k_up = exponent_for(__uint_as_float(own));
+        const Place at(tid);
+        if (at.k_eighth == 0) key_up_sh[u & 3][at.k_row] = (int8_t)k_up;
+        k_f = pow2(k_up);
+      } else {
+        // (A key of zeros has no bits to lose; 1 less, it is the largest of all.)
+        const uint32_t top = wave_max_of_eighths(own), least = wave_min_of_eighths(own - 1);
+        const int k_up = __builtin_amdgcn_readfirstlane(exponent_for(__uint_as_float(top)));
+        if (lane == 0) {
+          info_sh[u & 3].k_up[wave] = (int8_t)k_up;
+          if (top >> 23 > (least >> 23) + EVEN) uneven_sh = 1;
+        }
+        k_f = pow2(k_up);
+      }
       const int v_up = __builtin_amdgcn_readfirstlane(exponent_for(wave_max(v_top)));
-      if (lane == 0) info_sh[u & 3].k_up[wave] = (int8_t)k_up, info_sh[u & 3].v_up[wave] = (int8_t)v_up;
-      k_f = pow2(k_up);
+      if (lane == 0) info_sh[u & 3].v_up[wave] = (int8_t)v_up;
       v_f = pow2(v_up);
     }
     const Place p(afresh(tid));
@@ -1097,7 +1135,8 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
       }
     }
   };
-  auto multiply = [&](int u, bool careful) __attribute__((always_inline)) {
+  auto multiply = [&](int u, auto with_care) __attribute__((always_inline)) {
+    constexpr bool careful = decltype(with_care)::value;
     const int base = span.tile(u) * TN, parity = u & 1;
     // Tiles past all of the wave's rows, or before all their windows.
     if (!wave_ok || base > pos_hi || (base + TN - 1 <= below_lo && base >= d.sinks)) return;
@@ -1171,9 +1210,18 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
         back[i] = q_back;
         fall[i] = 0;
         if constexpr (SCALED) {
-          const int k_up = (int8_t)((tb ? ups[1] : ups[0]) >> 8 * i);
           // (Neither 0 nor infinity: a hidden score is -infinity, others may be 0.)
-          back[i] = __builtin_amdgcn_fmed3f(q_back * pow2(-k_up), 1.17549435e-38f, 3.402823466e38f);
+          const auto out_of = [&](int up) {
+            return __builtin_amdgcn_fmed3f(q_back * pow2(-up), 1.17549435e-38f, 3.402823466e38f);
+          };
+          if constexpr (careful) {
+            const uint32_t four = *(const uint32_t*)&key_up_sh[u & 3][32 * tb + 8 * i + 4 * h];
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[4 * i + e] *= out_of((int8_t)(four >> 8 * e));
+            back[i] = 1.f;
+          } else {
+            back[i] = out_of((int8_t)((tb ? ups[1] : ups[0]) >> 8 * i));
+          }
           fall[i] = max(o_up - (int)(int8_t)((tb ? ups[3] : ups[2]) >> 8 * i), -100);
         }
       }
@@ -1229,7 +1277,7 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
     }
   };
   // A tile's buffer, tops and flags go by the parity of its number.
-  auto pass = [&](bool careful) __attribute__((always_inline)) {
+  auto pass = [&](auto careful) __attribute__((always_inline)) {
     m = NEG_INF, l = 0.f;
     o_up = 113;  // as for values that are all zero or very small
     poison = false;
@@ -1245,6 +1293,7 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
       }
       load(u + 2);
     };
+    if (tid == 0) uneven_sh = 0;
     find_page(u0);
     find_rows(u0);
     find_page(u0 + 1);
@@ -1266,15 +1315,13 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
     }
     __syncthreads();
   };
-  for (int k = 0; k < 2; k++) {
-    pass(k);
-    bool bad = !finite(l);
+  pass(std::false_type{});
+  bool again = !finite(l);
 #pragma unroll
-    for (int b = 0; b < NB; b++)
+  for (int b = 0; b < NB; b++)
 #pragma unroll
-      for (int e = 0; e < 16; e++) bad |= !finite(o[b][e]);
-    if (!__syncthreads_or(bad && wave_ok)) break;
-  }
+    for (int e = 0; e < 16; e++) again |= !finite(o[b][e]);
+  if (__syncthreads_or((again && wave_ok) || uneven_sh)) pass(std::true_type{});
   l = half_sum(l);
   if (half_max(poison ? 1.f : 0.f) > 0.f) l = __builtin_nanf("");
   if (!row_ok) return;

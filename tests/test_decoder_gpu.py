@@ -958,3 +958,46 @@ def test_sample_infinite_temperature(rh, f, vocab):
         assert tokens[r] == kept[int(float(u[r]) * len(kept))], (r, tokens[r])
         want = -math.log(len(kept))
         assert abs(logprobs[r] - want) <= 2 * U * max(1.0, -want), (r, logprobs[r], want)
+
+
+@pytest.mark.parametrize("cache_type", TYPES)
+@pytest.mark.parametrize("hq,dim", [(1, 64), (4, 128), (1, 192)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf])
+def test_attention_infinite_keys_leave_their_neighbours(rh, cache_type, hq, dim, bad):
+    """An infinity in a key whose values are finite: the rows before the token
+    are as they are without it, also where the scores of those that see it
+    are -infinity and leave nothing that is not finite."""
+    for seed in range(4):
+        for q_len, kv, back in ((40, 90, 1), (33, 70, 2), (300, 300, 7)):
+            s = Paged([q_len], [kv], 16)
+            at = kv - back
+            p, o = s.place(0, at)
+
+            def tweak(q, k, v):
+                k[p, o, 0, 5] = bad
+
+            got, q, k, v, scale = run_attention(rh, s, hq, 1, dim, cache_type, tweak=tweak, seed=seed)
+            n = q_len - back  # rows before the token
+            s2 = Paged([n], [at], 16)
+            s2.table, s2.n_pages = s.table, s.n_pages
+            want, tol = attention_ref(q[:n], k, v, s2, scale, 0, 0)
+            attention_close(got[:n], want, tol, (seed, q_len, back))
+
+
+@pytest.mark.parametrize("cache_type", ["float32", "bfloat16"])
+@pytest.mark.parametrize("loud", [2.0 ** 13, 2.0 ** 20, 1e12, 1e30])
+@pytest.mark.parametrize("q_len,kv,window,sinks,dim", [(40, 90, 0, 0, 64), (200, 700, 0, 0, 128), (60, 150, 20, 3, 64),
+                                                       (30, 60, 0, 0, 256)])
+def test_attention_loud_keys_leave_their_neighbours(rh, cache_type, loud, q_len, kv, window, sinks, dim):
+    """Two keys that are far larger than the others, one that some rows do not
+    see yet and one that, with a window, later rows do not see any more."""
+    s = Paged([q_len], [kv], 16)
+
+    def tweak(q, k, v):
+        for at in [kv - 3] + ([kv - q_len - 10] if window else []):
+            p, o = s.place(0, at)
+            k[p, o] *= loud
+
+    got, q, k, v, scale = run_attention(rh, s, 2, 1, dim, cache_type, window, sinks, tweak=tweak)
+    want, tol = attention_ref(q, k, v, s, scale, window, sinks)
+    attention_close(got, want, tol)
