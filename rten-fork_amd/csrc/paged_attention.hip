@@ -31,6 +31,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -267,7 +268,23 @@ __device__ __forceinline__ uint32_t wave_min_of_eighths(uint32_t x) {
   const auto s = __builtin_amdgcn_permlane32_swap(x, x, false, false);
   return min(s[0], s[1]);
 }
-__device__ __forceinline__ float wave_max(float y) { return __uint_as_float(wave_max_of_eighths(eighth_max(y))); }
+__device__ __forceinline__ uint32_t wave_min(uint32_t x) {
+  x = min(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 0xF, 0xF, true));
+  x = min(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xF, 0xF, true));
+  x = min(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x141, 0xF, 0xF, true));
+  return wave_min_of_eighths(x);
+}
+// The largest, over every 32 lanes, of the lanes' two 16-bit numbers each.
+__device__ __forceinline__ u16x2 half_max16(u16x2 x) {
+  const auto step = [](u16x2 a, int b) { return __builtin_elementwise_max(a, __builtin_bit_cast(u16x2, b)); };
+  x = step(x, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0xB1, 0xF, 0xF, true));
+  x = step(x, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x4E, 0xF, 0xF, true));
+  x = step(x, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x141, 0xF, 0xF, true));
+  x = step(x, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x140, 0xF, 0xF, true));
+  const uint32_t y = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane16_swap(y, y, false, false);
+  return step(__builtin_bit_cast(u16x2, (uint32_t)r[0]), (int)r[1]);
+}
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
@@ -301,10 +318,10 @@ __device__ __forceinline__ void split16(float a, float b, float minus1, f16x2& h
   hi = opaque((f16x2){(_Float16)a, (_Float16)b});
   lo = (f16x2){(_Float16)__builtin_fmaf((float)hi[0], minus1, a), (_Float16)__builtin_fmaf((float)hi[1], minus1, b)};
 }
-// The same of a f and b f, f a power of two.
-__device__ __forceinline__ void split16(float a, float b, float f, float minus1, f16x2& hi, f16x2& lo) {
-  hi = opaque((f16x2){(_Float16)(a * f), (_Float16)(b * f)});
-  lo = (f16x2){(_Float16)__builtin_fmaf(a, f, -(float)hi[0]), (_Float16)__builtin_fmaf(b, f, -(float)hi[1])};
+// The same of a f and b g, f and g powers of two.
+__device__ __forceinline__ void split16(float a, float b, float f, float g, f16x2& hi, f16x2& lo) {
+  hi = opaque((f16x2){(_Float16)(a * f), (_Float16)(b * g)});
+  lo = (f16x2){(_Float16)__builtin_fmaf(a, f, -(float)hi[0]), (_Float16)__builtin_fmaf(b, g, -(float)hi[1])};
 }
 
 template <int TYPE>
@@ -772,10 +789,14 @@ __global__ __launch_bounds__(PA_THREADS, (DecodeTile<DP, TYPE>::WAVES)) void dec
 //    out again exactly: a score is multiplied by its keys' and its row's on
 //    its way into the exponential, whose argument takes the values'.
 //    Not all rows see all of 8 keys, and a loud one must not cost its
-//    neighbours their bits: where the largest numbers of 8 keys are more than
-//    2^EVEN apart (an infinity always is), the stretch is computed again with a
-//    power of two for each key (careful).  Up to there a key is exact to 2^-26
-//    of its own largest number, which is finer than the split's 22 bits.
+//    neighbours their bits: where the largest numbers of 8 keys, or of their
+//    values, are more than 2^EVEN apart (an infinity always is), or values more
+//    than 2^FALL below the loudest before them or in their tile, the stretch is
+//    computed again with a power of two for each key and each value's row, and
+//    the products of values of different loudness apart (careful).  Up to there
+//    a row is exact to 2^-26 of its own largest number and p to 2^-23 of the
+//    largest p, finer than the split's 22 bits.  (Values below 2^-94 can vanish
+//    beside others above 2^53 in either pass.)
 //  - S^T = K Q^T: a lane (n, h) has row n's scores for the keys
 //    8 i + 4 h + j of each 32, so the softmax needs one exchange with lane
 //    ^ 32, and
@@ -863,8 +884,12 @@ struct __attribute__((aligned(16))) TileInfo {
 };
 
 // How many binades the largest numbers of 8 keys may lie apart to share an
-// exponent.
+// exponent, how many the values of a tile below the result's scale, and that
+// scale's least exponent (no sum of 2^127s that counts overflows, and there are
+// 85 binades below 1).
 constexpr uint32_t EVEN = 12;
+constexpr int FALL = 10, O_LEAST = -41;
+constexpr int NO_VALUE = 127;  // the exponent of values that are all zero (or below 2^-133)
 
 // x, of which the compiler does not know that it is the same in every round of
 // a loop: what follows from it is formed again there, a few instructions,
@@ -906,7 +931,8 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
   // [tile & 3], as they are read late.
   __shared__ int64_t rows_sh[4][2][TN];  // the keys' and the values' rows
   __shared__ TileInfo info_sh[4];
-  __shared__ __attribute__((aligned(4))) int8_t key_up_sh[SCALED ? 4 : 1][TN];  // each key's exponent, with care
+  // Each key's exponent and its value's, with care.
+  __shared__ __attribute__((aligned(4))) int8_t key_up_sh[SCALED ? 4 : 1][TN], value_up_sh[SCALED ? 4 : 1][TN];
   __shared__ int uneven_sh;
   Work w;
   if (!plan<true, T::THREADS, T::ROWS>(d, blockIdx.x, plan_sh, w) || w.slot >= d.slots_big) return;
@@ -1015,7 +1041,7 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
   float m, l;
   f32x16 o[NB];
   int o_up;  // o is 2^o_up times the result
-  bool poison;
+  bool poison, uneven = false;
   // Converts the tile in the registers into its buffer.
   auto stage = [&](int u, auto with_care) __attribute__((always_inline)) {
     constexpr bool careful = decltype(with_care)::value;
@@ -1047,9 +1073,9 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
         if (bad) atomicOr((unsigned long long*)&info_sh[u & 3].bad, 1ull << (Place(tid).v_key + r));
       }
     }
-    float k_f = 1.f, v_f = 1.f;
+    float k_f = 1.f, v_f[4] = {1.f, 1.f, 1.f, 1.f};
     if constexpr (SCALED) {
-      float k_top = 0.f, v_top = 0.f;
+      float k_top = 0.f, v_top[4] = {0.f, 0.f, 0.f, 0.f};
       if constexpr (careful) {
 #pragma unroll
         for (int j = 0; j < KL; j++)
@@ -1066,10 +1092,9 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
           for (int e = 0; e < 4; e += 2) k_top = top_of<TYPE>(k_top, k_in[j][e], k_in[j][e + 1]);
       }
 #pragma unroll
-      for (int c = 0; c < VW; c++) {
-        v_top = top_of<TYPE>(v_top, v_in[0][c], v_in[1][c]);
-        v_top = top_of<TYPE>(v_top, v_in[2][c], v_in[3][c]);
-      }
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int c = 0; c < VW; c += 2) v_top[r] = top_of<TYPE>(v_top[r], v_in[r][c], c + 1 < VW ? v_in[r][c + 1] : 0);
       const uint32_t own = eighth_max(k_top);  // the lane's key's
       if constexpr (careful) {
         const int k_up = exponent_for(__uint_as_float(own));
@@ -1086,9 +1111,44 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
         }
         k_f = pow2(k_up);
       }
-      const int v_up = __builtin_amdgcn_readfirstlane(exponent_for(wave_max(v_top)));
-      if (lane == 0) info_sh[u & 3].v_up[wave] = (int8_t)v_up;
-      v_f = pow2(v_up);
+      // (Of the values' tops the upper halves do: exponents and seven bits.)
+      const auto two = [](float a, float b) {
+        return half_max16(
+            __builtin_bit_cast(u16x2, __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u)));
+      };
+      const u16x2 tops[2] = {two(v_top[0], v_top[1]), two(v_top[2], v_top[3])};
+      const auto value_up = [](uint32_t top) {
+        return top ? exponent_for(__uint_as_float(top << 16)) : NO_VALUE;
+      };
+      const auto factor = [](int up) { return up == NO_VALUE ? 0.f : pow2(up); };
+      if constexpr (careful) {
+        const Place at(tid);
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int v_up = value_up(tops[r / 2][r % 2]);
+          if (at.v_group == 0) value_up_sh[u & 3][at.v_key + r] = (int8_t)v_up;
+          v_f[r] = factor(v_up);
+        }
+      } else {
+        const auto other = [](u16x2 x) {
+          const uint32_t y = __builtin_bit_cast(uint32_t, x);
+          return __builtin_amdgcn_permlane32_swap(y, y, false, false);
+        };
+        const auto a = other(__builtin_elementwise_max(tops[0], tops[1]));
+        const auto b = other(__builtin_elementwise_min(tops[0] - (uint16_t)1, tops[1] - (uint16_t)1));
+        const u16x2 most = __builtin_elementwise_max(__builtin_bit_cast(u16x2, (uint32_t)a[0]),
+                                                     __builtin_bit_cast(u16x2, (uint32_t)a[1]));
+        const u16x2 least = __builtin_elementwise_min(__builtin_bit_cast(u16x2, (uint32_t)b[0]),
+                                                      __builtin_bit_cast(u16x2, (uint32_t)b[1]));
+        const uint32_t top = __builtin_amdgcn_readfirstlane(max((uint32_t)most[0], (uint32_t)most[1]));
+        const int v_up = value_up(top);
+        if (lane == 0) {
+          info_sh[u & 3].v_up[wave] = (int8_t)v_up;
+          if (top >> 7 > (min((uint32_t)least[0], (uint32_t)least[1]) >> 7) + EVEN) uneven_sh = 1;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) v_f[r] = factor(v_up);
+      }
     }
     const Place p(afresh(tid));
     char* kt = &buffer_sh[parity][p.k_row * KS];
@@ -1106,8 +1166,8 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
         *(u32x4*)(kt + at) = y;
       } else {
         f16x2 h0, l0, h1, l1;
-        split16(__uint_as_float(k_in[j][0]), __uint_as_float(k_in[j][1]), k_f, d.minus1, h0, l0);
-        split16(__uint_as_float(k_in[j][2]), __uint_as_float(k_in[j][3]), k_f, d.minus1, h1, l1);
+        split16(__uint_as_float(k_in[j][0]), __uint_as_float(k_in[j][1]), k_f, k_f, h0, l0);
+        split16(__uint_as_float(k_in[j][2]), __uint_as_float(k_in[j][3]), k_f, k_f, h1, l1);
         *(f16x4*)(kt + at) = (f16x4){h0[0], h0[1], h1[0], h1[1]};
         *(f16x4*)(kt + T::K_BYTES + at) = (f16x4){l0[0], l0[1], l1[0], l1[1]};
       }
@@ -1124,16 +1184,26 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
         float x[4];
 #pragma unroll
         for (int r = 0; r < 4; r++)
-          x[r] = (e & 1 ? cache_hi<TYPE>(v_in[r][e / 2]) : cache_lo<TYPE>(v_in[r][e / 2])) * v_f;
+          x[r] = (e & 1 ? cache_hi<TYPE>(v_in[r][e / 2]) : cache_lo<TYPE>(v_in[r][e / 2])) * v_f[r];
         *(f16x4*)(vt + at) = (f16x4){(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
       } else {
         f16x2 h0, l0, h1, l1;
-        split16(__uint_as_float(v_in[0][e]), __uint_as_float(v_in[1][e]), v_f, d.minus1, h0, l0);
-        split16(__uint_as_float(v_in[2][e]), __uint_as_float(v_in[3][e]), v_f, d.minus1, h1, l1);
+        split16(__uint_as_float(v_in[0][e]), __uint_as_float(v_in[1][e]), v_f[0], v_f[1], h0, l0);
+        split16(__uint_as_float(v_in[2][e]), __uint_as_float(v_in[3][e]), v_f[2], v_f[3], h1, l1);
         *(f16x4*)(vt + at) = (f16x4){h0[0], h0[1], h1[0], h1[1]};
         *(f16x4*)(vt + T::V_BYTES + at) = (f16x4){l0[0], l0[1], l1[0], l1[1]};
       }
     }
+  };
+  // Gives o a smaller power of two.
+  auto rescale = [&](int up) __attribute__((always_inline)) {
+    const int to = max(up, O_LEAST), by = to - o_up;
+    if (by >= 0) return;
+    o_up = to;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int e = 0; e < 16; e++) o[b][e] = __builtin_amdgcn_ldexpf(o[b][e], by);
   };
   auto multiply = [&](int u, auto with_care) __attribute__((always_inline)) {
     constexpr bool careful = decltype(with_care)::value;
@@ -1150,18 +1220,12 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
         ups[i] = __builtin_amdgcn_readfirstlane(ups[i]), keys[i] = __builtin_amdgcn_readfirstlane(keys[i]);
       whole = (keys[0] & (TN == 64 ? keys[1] : ~0u)) == ~0u && !careful && wave_row + 31 < all_rows &&
               base + TN - 1 <= pos_lo && (base > below_hi || base + TN <= d.sinks);
-      if constexpr (SCALED) {
-        int least = 127;
+      if constexpr (SCALED && !careful) {
+        int least = NO_VALUE;
 #pragma unroll
         for (int i = 0; i < WAVES; i++) least = min(least, (int)(int8_t)(ups[2 + i / 4] >> 8 * (i % 4)));
-        if (least < o_up) {  // larger values than any before: a binade more of room
-          const float f = pow2(least - 1 - o_up);
-          o_up = least - 1;
-#pragma unroll
-          for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) o[b][e] *= f;
-        }
+        if (least < o_up) rescale(least - 1);  // larger values than any before: a binade more of room
+        uneven |= least < o_up;
       }
     };
     const char* ks = buffer_sh[parity];
@@ -1200,9 +1264,7 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
         }
         if (careful) poison |= (seen & (tb ? keys[3] : keys[2]) >> 4 * half) != 0;
       }
-      // The factors of every 8 keys: of their scores, and of p.  (Values that
-      // are 2^100 below the largest may as well be a little larger; their p
-      // still counts in l.)
+      // The factors of every 8 keys: of their scores, and of p.
       float back[4];
       int fall[4];
 #pragma unroll
@@ -1222,7 +1284,11 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
           } else {
             back[i] = out_of((int8_t)((tb ? ups[1] : ups[0]) >> 8 * i));
           }
-          fall[i] = max(o_up - (int)(int8_t)((tb ? ups[3] : ups[2]) >> 8 * i), -100);
+          if constexpr (!careful) {
+            const int up = (int8_t)((tb ? ups[3] : ups[2]) >> 8 * i);
+            fall[i] = up == NO_VALUE ? 0 : max(o_up - up, -FALL);
+            uneven |= up != NO_VALUE && o_up - up < -FALL;
+          }
         }
       }
       float top = NEG_INF;
@@ -1243,6 +1309,55 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
       // p 2^8: at most 2^14.
       const float ref = 8.f - (m == NEG_INF ? 0.f : m);
       f16x8 p_hi[2], p_lo[2];
+      if constexpr (SCALED && careful) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(s[e] + ref), l += s[e];
+        // The loudest values left and those within 2^FALL of them, until there
+        // are none.
+        const int own_up = value_up_sh[u & 3][32 * tb + n];
+        uint32_t left = (uint32_t)__ballot(own_up != NO_VALUE);
+        while (left) {
+          const int up = __builtin_amdgcn_readfirstlane((int)wave_min(left >> n & 1 ? own_up + 128 : 255)) - 128;
+          const uint32_t now = (uint32_t)__ballot((left >> n & 1) && own_up <= up + FALL);
+          left &= ~now;
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const uint32_t four = *(const uint32_t*)&value_up_sh[u & 3][32 * tb + 8 * i + 4 * h];
+            const uint32_t here = now >> (8 * i + 4 * h);
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              p[e] = here >> e & 1 ? __builtin_amdgcn_ldexpf(s[4 * i + e], up - (int)(int8_t)(four >> 8 * e)) : 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+              f16x2 hi, lo;
+              split16(p[e], p[e + 1], d.minus1, hi, lo);
+              const int at = 4 * (i & 1) + e;
+              p_hi[i / 2][at] = hi[0], p_hi[i / 2][at + 1] = hi[1];
+              p_lo[i / 2][at] = lo[0], p_lo[i / 2][at + 1] = lo[1];
+            }
+          }
+          rescale(up - 1);
+#pragma unroll
+          for (int b = 0; b < NB; b++) {
+            f32x16 t;
+#pragma unroll
+            for (int e = 0; e < 16; e++) t[e] = 0.f;
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+              const int at = (v_base ^ value_flip<TN>(32 * b, 2 * (2 * tb + c))) + 32 * b * TN * 2;
+              const f16x8 x = *(const f16x8*)(vs + at);
+              t = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p_hi[c], t, 0, 0, 0);
+              t = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p_lo[c], t, 0, 0, 0);
+              if constexpr (TERMS == 2)
+                t = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const f16x8*)(vs + T::V_BYTES + at), p_hi[c], t, 0, 0, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[b][e] += __builtin_amdgcn_ldexpf(t[e], o_up - up);
+          }
+        }
+        continue;
+      }
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const float at = ref + (float)fall[i];
@@ -1309,19 +1424,20 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
       // Tile u is in its buffer, u + 2's rows are there, and nobody reads u - 1
       // any more.
       __syncthreads();
-      if (wave < 4) advance(u);
+      if (WAVES == 4 || wave < 4) advance(u);
       multiply(u, careful);
-      if (wave >= 4) advance(u);
+      if (WAVES == 8 && wave >= 4) advance(u);
     }
     __syncthreads();
   };
   pass(std::false_type{});
-  bool again = !finite(l);
+  bool again = uneven || !finite(l);
 #pragma unroll
   for (int b = 0; b < NB; b++)
 #pragma unroll
     for (int e = 0; e < 16; e++) again |= !finite(o[b][e]);
-  if (__syncthreads_or((again && wave_ok) || uneven_sh)) pass(std::true_type{});
+  // (Seldom: what does not fit the registers is kept elsewhere there, not here.)
+  if (__builtin_expect(__syncthreads_or((again && wave_ok) || uneven_sh) != 0, 0)) pass(std::true_type{});
   l = half_sum(l);
   if (half_max(poison ? 1.f : 0.f) > 0.f) l = __builtin_nanf("");
   if (!row_ok) return;

@@ -1001,3 +1001,42 @@ def test_attention_loud_keys_leave_their_neighbours(rh, cache_type, loud, q_len,
     got, q, k, v, scale = run_attention(rh, s, 2, 1, dim, cache_type, window, sinks, tweak=tweak)
     want, tol = attention_ref(q, k, v, s, scale, window, sinks)
     attention_close(got, want, tol)
+
+
+@pytest.mark.parametrize("cache_type", ["float32", "bfloat16"])
+@pytest.mark.parametrize("loud", [2.0 ** 9, 2.0 ** 11, 2.0 ** 14, 2.0 ** 20, 1e12, 1e30])
+@pytest.mark.parametrize("q_len,kv,window,sinks,dim", [(40, 90, 0, 0, 64), (200, 700, 0, 0, 128), (60, 150, 20, 3, 64),
+                                                       (30, 60, 0, 0, 256), (300, 300, 0, 0, 96)])
+def test_attention_loud_values_leave_their_neighbours(rh, cache_type, loud, q_len, kv, window, sinks, dim):
+    """Values far larger than the others: of a token that some rows do not see
+    yet, of a whole tile of such tokens, and, with a window, of tokens that
+    later rows do not see any more."""
+    s = Paged([q_len], [kv], 16)
+    for where in ([kv - 3], range(kv - 20, kv), range(kv - q_len - 10, kv - q_len - 8) if window else [2]):
+        def tweak(q, k, v):
+            for at in where:
+                p, o = s.place(0, at)
+                v[p, o] *= loud
+
+        got, q, k, v, scale = run_attention(rh, s, 2, 1, dim, cache_type, window, sinks, tweak=tweak)
+        want, tol = attention_ref(q, k, v, s, scale, window, sinks)
+        attention_close(got, want, tol, (loud, where))
+
+
+@pytest.mark.parametrize("cache_type", ["float32", "bfloat16"])
+@pytest.mark.parametrize("spread", [6, 30, 90])
+def test_attention_values_of_all_sizes(rh, cache_type, spread):
+    """Keys' values from 2^-spread to 2^spread, some all zero, in two sequences
+    of which one is cut."""
+    import torch
+
+    s = Paged([50, 20], [1500, 70], 16)
+
+    def tweak(q, k, v):
+        g = torch.Generator().manual_seed(spread)
+        v *= torch.exp2(torch.randint(-spread, spread + 1, v.shape[:3], generator=g).float())[..., None].to(v.dtype)
+        v[torch.rand(v.shape[:3], generator=g) < 0.1] = 0
+
+    got, q, k, v, scale = run_attention(rh, s, 4, 2, 64, cache_type, tweak=tweak)
+    want, tol = attention_ref(q, k, v, s, scale, 0, 0)
+    attention_close(got, want, tol)
