@@ -1280,7 +1280,6 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
             const uint32_t four = *(const uint32_t*)&key_up_sh[u & 3][32 * tb + 8 * i + 4 * h];
 #pragma unroll
             for (int e = 0; e < 4; e++) s[4 * i + e] *= out_of((int8_t)(four >> 8 * e));
-            back[i] = 1.f;
           } else {
             back[i] = out_of((int8_t)((tb ? ups[1] : ups[0]) >> 8 * i));
           }
@@ -1291,13 +1290,26 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
           }
         }
       }
+      if constexpr (careful) {  // the scores themselves
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          if constexpr (!SCALED) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[4 * i + e] *= q_back;
+          }
+          back[i] = 1.f;
+        }
+      }
       float top = NEG_INF;
 #pragma unroll
       for (int i = 0; i < 4; i++)
         top = fmaxf(top, fmaxf(fmaxf(s[4 * i], s[4 * i + 1]), fmaxf(s[4 * i + 2], s[4 * i + 3])) * back[i]);
       top = half_max(top);
-      if (__any(top > m + 6.f)) {
+      if (__any(careful ? top - m > 6.f : top > m + 6.f)) {
         const float m_new = fmaxf(m, top);
+        // Neither 8 - m nor m + 6 is exact any more: with care the difference to
+        // m is taken first.
+        uneven |= fabsf(m_new) > 4194304.f && m_new != NEG_INF;
         const float fade = __builtin_amdgcn_exp2f(m - (m_new == NEG_INF ? 0.f : m_new));
         m = m_new;
         l *= fade;
@@ -1307,11 +1319,11 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
           for (int e = 0; e < 16; e++) o[b][e] *= fade;
       }
       // p 2^8: at most 2^14.
-      const float ref = 8.f - (m == NEG_INF ? 0.f : m);
+      const float m_of = m == NEG_INF ? 0.f : m, ref = 8.f - m_of;
       f16x8 p_hi[2], p_lo[2];
       if constexpr (SCALED && careful) {
 #pragma unroll
-        for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f(s[e] + ref), l += s[e];
+        for (int e = 0; e < 16; e++) s[e] = __builtin_amdgcn_exp2f((s[e] - m_of) + 8.f), l += s[e];
         // The loudest values left and those within 2^FALL of them, until there
         // are none.
         const int own_up = value_up_sh[u & 3][32 * tb + n];
@@ -1364,8 +1376,8 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
         float sum = 0.f;
 #pragma unroll
         for (int e = 4 * i; e < 4 * i + 4; e += 2) {
-          const float a = __builtin_amdgcn_exp2f(__fmaf_rn(s[e], back[i], at));
-          const float b = __builtin_amdgcn_exp2f(__fmaf_rn(s[e + 1], back[i], at));
+          const float a = __builtin_amdgcn_exp2f(careful ? (s[e] - m_of) + 8.f : __fmaf_rn(s[e], back[i], at));
+          const float b = __builtin_amdgcn_exp2f(careful ? (s[e + 1] - m_of) + 8.f : __fmaf_rn(s[e + 1], back[i], at));
           sum += a + b;
           f16x2 hi, lo;
           split16(a, b, d.minus1, hi, lo);

@@ -1040,3 +1040,39 @@ def test_attention_values_of_all_sizes(rh, cache_type, spread):
     got, q, k, v, scale = run_attention(rh, s, 4, 2, 64, cache_type, tweak=tweak)
     want, tol = attention_ref(q, k, v, s, scale, 0, 0)
     attention_close(got, want, tol)
+
+
+@pytest.mark.parametrize("cache_type", TYPES)
+@pytest.mark.parametrize("hq,hk,dim,q_len", [(8, 1, 64, 1), (2, 1, 64, 40), (3, 1, 128, 70), (1, 1, 256, 33)])
+@pytest.mark.parametrize("base", [2.0 ** 21, 2.0 ** 24, 2.0 ** 25, 2.0 ** 26, 2.0 ** 27, -2.0 ** 26, -2.0 ** 27])
+def test_attention_scores_of_few_bits_behind_the_point(rh, cache_type, hq, hk, dim, q_len, base):
+    """Scores so large that whole numbers are rounded, rising by one step of
+    float32 from one stretch of keys to the next, all sums exact."""
+    import torch
+
+    kv = 200
+    s = Paged([q_len], [kv], 16)
+    # scale log2 e is 1: the weights are powers of two.
+    scale = np.float32(math.log(2))
+    assert scale * np.float32(1.44269504088896340736) == 1
+    step = 2.0 ** max(0, int(math.log2(abs(base))) - 23)
+    root = 2.0 ** 12
+    rise = np.arange(kv) // 30
+
+    def tweak(q, k, v):
+        q.zero_()
+        q[..., 0], q[..., 1] = abs(base) / root, step
+        k.zero_()
+        for j in range(kv):
+            p, o = s.place(0, j)
+            k[p, o, :, 0], k[p, o, :, 1] = math.copysign(root, base), float(rise[j])
+
+    got, q, k, v, _ = run_attention(rh, s, hq, hk, dim, cache_type, tweak=tweak, scale=float(scale))
+    vv = np.stack([v[s.place(0, j)] for j in range(kv)])[:, 0].astype(np.float64)
+    for t in range(q_len):
+        n = kv - q_len + t + 1
+        w = np.exp2((rise[:n] - rise[n - 1]) * step)
+        want = (w / w.sum()) @ vv[:n]
+        # (The sums over the keys, the split of p and v, the powers and the
+        # quotient: as attention_ref counts them.)
+        assert (np.abs(got[t] - want) <= (n / 16 + 40) * U * np.abs(vv[:n]).max()).all(), t
