@@ -1458,7 +1458,8 @@ __global__ __launch_bounds__((ChunkTile<DP, TYPE>::THREADS), DP == 256 ? 1 : 2) 
   const int r = afresh(wave * 32 + n), to_token = fdiv(row0 + r, d.group_div), to_sub = row0 + r - to_token * d.group;
   float* to = w.slot < 0 ? d.out + (int64_t)(w.start + to_token) * d.o_t + (int64_t)(w.head * d.group + to_sub) * d.o_h
                          : d.o_big + ((int64_t)w.slot * T::ROWS + r) * dim;
-  if (w.slot >= 0 && h == 0) d.ml_big[(int64_t)w.slot * T::ROWS + r] = make_float2(m, l);
+  // (Without p's 2^14: results times weights of up to 1 are summed in 32 bits.)
+  if (w.slot >= 0 && h == 0) d.ml_big[(int64_t)w.slot * T::ROWS + r] = make_float2(m, l * 0x1p-14f);
 #pragma unroll
   for (int b = 0; b < NB; b++)
 #pragma unroll

@@ -1076,3 +1076,17 @@ def test_attention_scores_of_few_bits_behind_the_point(rh, cache_type, hq, hk, d
         # (The sums over the keys, the split of p and v, the powers and the
         # quotient: as attention_ref counts them.)
         assert (np.abs(got[t] - want) <= (n / 16 + 40) * U * np.abs(vv[:n]).max()).all(), t
+
+
+@pytest.mark.parametrize("q_len", [1, 40])
+def test_attention_joins_values_near_the_end_of_the_range(rh, q_len):
+    """A float32 cache's values at 2^-12 of the largest number, in a sequence
+    that is cut into stretches."""
+    s = Paged([q_len], [2000], 16)
+
+    def tweak(q, k, v):
+        v *= 3e35 / 4
+
+    got, q, k, v, scale = run_attention(rh, s, 2, 1, 64, "float32", tweak=tweak)
+    want, tol = attention_ref(q, k, v, s, scale, 0, 0)
+    attention_close(got, want, tol)
