@@ -284,13 +284,17 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ctx
         raise OpError(3, "Expected [rows, vocab] logits")
     rows, vocab = logits.shape
 
-    def per_row(value, dtype, what):
-        return _vector(value, rows, ctx, dtype, what) if isinstance(value, torch.Tensor) else 0
+    def per_row(value, none, dtype, what):
+        """(The number for all rows, the address of those of each.)"""
+        if isinstance(value, torch.Tensor):
+            return none, _vector(value, rows, ctx, dtype, what)
+        return value, 0
 
-    t, k = per_row(temperature, f32, "temperature"), per_row(top_k, i32, "top_k")
-    p, m = per_row(top_p, f32, "top_p"), per_row(min_p, f32, "min_p")
-    s = _SAMPLING.pack(1. if t else temperature, 1. if p else top_p, 0. if m else min_p,
-                       0 if k else min(max(int(top_k), 0), vocab), t, p, m, k)
+    t, ts = per_row(temperature, 1., f32, "temperature")
+    k, ks = per_row(top_k, 0, i32, "top_k")
+    p, ps = per_row(top_p, 1., f32, "top_p")
+    m, ms = per_row(min_p, 0., f32, "min_p")
+    s = _SAMPLING.pack(t, p, m, min(max(int(k), 0), vocab), ts, ps, ms, ks)
     u = _vector(uniforms, rows, ctx, f32, "uniforms")
     need = _sample_workspace(rows, vocab)
     tokens, logprobs = _empty(logits, (rows,), i32, ctx, here), _empty(logits, (rows,), f32, ctx, here)

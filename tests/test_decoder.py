@@ -292,6 +292,26 @@ def test_python_binding_refuses_before_the_library(d):
             d._cache(k, v, Ctx)
 
 
+class NoGPU:
+    """A context of the CPU: a call gets as far as the library's own check of it."""
+    device, ptr, stream = -1, None, None
+
+
+@pytest.fixture
+def on_cpu(d, monkeypatch):
+    monkeypatch.setattr(d, "_context", lambda ctx: (NoGPU, True))
+    return d
+
+
+@pytest.mark.parametrize("each", ["temperature", "top_k", "top_p", "min_p"])
+def test_sample_no_rows(on_cpu, each):
+    """Filters of each of no rows."""
+    torch = pytest.importorskip("torch")
+    none = torch.empty(0, dtype=torch.int32 if each == "top_k" else torch.float32)
+    tokens, logprobs = on_cpu.sample(torch.zeros(0, 10), torch.zeros(0), **{each: none})
+    assert tokens.shape == logprobs.shape == (0,)
+
+
 def test_packed_descriptors_have_the_structures_layouts(d):
     """The bytes that the binding passes, field by field."""
     def same(kind, packed, **fields):
