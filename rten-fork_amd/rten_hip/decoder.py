@@ -70,6 +70,7 @@ _CACHE = struct.Struct("PPiiqii3q3q")
 _SEQUENCES = struct.Struct("PqPPii")
 _ROTARY = struct.Struct("PPPPfii4x")
 _SAMPLING = struct.Struct("fffiPPPP")
+_FLOAT_MAX = 3.4028234663852886e38
 
 
 def _call(name, *args):
@@ -185,6 +186,8 @@ def _rotary(inv_freq, positions, tokens, dim, q_scale, k_scale, epsilon, interle
         half = inv_freq.shape[0]
         if half > 128:
             raise OpError(6, "rotary_dim must be a multiple of 8 up to head_dim")
+    if _FLOAT_MAX < epsilon < math.inf:
+        raise OpError(5, "epsilon must be a float32 number")
     return _ROTARY.pack(_vector(q_scale, dim, ctx, f32, "q_scale"), _vector(k_scale, dim, ctx, f32, "k_scale"),
                         _vector(inv_freq, half, ctx, f32, "inv_freq"),
                         _vector(positions, tokens, ctx, torch.int32, "positions"), epsilon, 2 * half,
@@ -288,7 +291,7 @@ def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ctx
         """(The number for all rows, the address of those of each.)"""
         if isinstance(value, torch.Tensor):
             return none, _vector(value, rows, ctx, dtype, what)
-        return value, 0
+        return value if dtype is i32 else C.c_float(value).value, 0  # (past its range: infinity)
 
     t, ts = per_row(temperature, 1., f32, "temperature")
     k, ks = per_row(top_k, 0, i32, "top_k")

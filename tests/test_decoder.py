@@ -312,6 +312,23 @@ def test_sample_no_rows(on_cpu, each):
     assert tokens.shape == logprobs.shape == (0,)
 
 
+def test_numbers_past_float32(on_cpu):
+    """They reach the library as infinities, or are refused as it refuses them."""
+    torch = pytest.importorskip("torch")
+    from rten_hip import OpError
+
+    for kw in (dict(temperature=1e39), dict(top_p=1e300), dict(min_p=-1e39), dict(temperature=-math.inf, min_p=1e39)):
+        with pytest.raises(OpError, match="Missing context"):
+            on_cpu.sample(torch.zeros(2, 10), torch.zeros(2), **kw)
+    x = torch.zeros(2, 1, 64)
+    for epsilon, text in ((1e39, "epsilon"), (-1e-9, "epsilon"), (math.inf, "Missing context")):
+        with pytest.raises(OpError, match=text):
+            on_cpu.qk_norm_rotary(x, x, torch.zeros(2, dtype=torch.int32), None, epsilon=epsilon)
+    n = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(OpError, match="scale must be finite"):
+        on_cpu.paged_attention(x, torch.zeros(3, 16, 1, 64), torch.zeros(3, 16, 1, 64), n[:, None], n, scale=1e39)
+
+
 def test_packed_descriptors_have_the_structures_layouts(d):
     """The bytes that the binding passes, field by field."""
     def same(kind, packed, **fields):
