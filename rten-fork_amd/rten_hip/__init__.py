@@ -229,15 +229,18 @@ def cpu_counts():
     return lg.value, ph.value
 
 
-_default_ctx: Optional[Context] = None
+_default = threading.local()
 
 
 def default_context() -> Context:
-    global _default_ctx
-    if _default_ctx is None:
-        _default_ctx = Context(0)
-    _default_ctx.sync_stream()
-    return _default_ctx
+    """The calling thread's own context on GPU 0, on torch's current stream of
+    that thread.  (One for all threads would queue a thread's work on the stream
+    that another one set last, with outputs and workspaces of its own.)"""
+    ctx = getattr(_default, "ctx", None)
+    if ctx is None:
+        ctx = _default.ctx = Context(0)
+    ctx.sync_stream()
+    return ctx
 
 
 def describe_i32(t) -> Tensor:

@@ -11,7 +11,9 @@ sequences, one after the other: ``q_starts[s]`` .. ``q_starts[s + 1]`` - 1 for
 sequence s; without ``q_starts`` row s is the one new token of sequence s.
 Rows from ``q_starts[-1]`` on are padding and left as they are.  ``kv_lens``
 counts the new tokens: append before attending.  All calls only queue work on
-the context's stream and can be captured.
+the context's stream and can be captured.  Without ``ctx`` that is the calling
+thread's own context on torch's current stream; a context that is given is used
+by one thread at a time.
 """
 from __future__ import annotations
 

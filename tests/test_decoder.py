@@ -329,6 +329,44 @@ def test_numbers_past_float32(on_cpu):
         on_cpu.paged_attention(x, torch.zeros(3, 16, 1, 64), torch.zeros(3, 16, 1, 64), n[:, None], n, scale=1e39)
 
 
+def test_default_context_of_each_thread(monkeypatch):
+    """Two threads on two streams: each one's calls stay on its own, however
+    they interleave."""
+    import threading
+
+    import rten_hip
+
+    here = threading.local()
+
+    class Recorder:  # a context that notes the stream it was set to last
+        def __init__(self, device):
+            self.device, self.stream = device, None
+
+        def sync_stream(self):
+            self.stream = here.stream
+
+    monkeypatch.setattr(rten_hip, "Context", Recorder)
+    if hasattr(rten_hip, "_default_ctx"):
+        monkeypatch.setattr(rten_hip, "_default_ctx", None)
+    turn, seen = threading.Barrier(2, timeout=20), {}
+
+    def work(name):
+        here.stream = name
+        ctx = rten_hip.default_context()
+        turn.wait()  # both have set their stream
+        seen[name] = (ctx, ctx.stream, rten_hip.default_context())
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in "ab"]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(30)
+    for name in "ab":
+        ctx, stream, again = seen[name]
+        assert stream == name and again is ctx
+    assert seen["a"][0] is not seen["b"][0]
+
+
 def test_packed_descriptors_have_the_structures_layouts(d):
     """The bytes that the binding passes, field by field."""
     def same(kind, packed, **fields):

@@ -1090,3 +1090,38 @@ def test_attention_joins_values_near_the_end_of_the_range(rh, q_len):
     got, q, k, v, scale = run_attention(rh, s, 2, 1, 64, "float32", tweak=tweak)
     want, tol = attention_ref(q, k, v, s, scale, 0, 0)
     attention_close(got, want, tol)
+
+
+def test_decoder_threads(rh):
+    """Two threads, each with its stream as torch's current one and without a
+    context of its own: the bits of the eager steps."""
+    import threading
+
+    import torch
+
+    steps = [Step(rh, 5, [300, 31]), Step(rh, 6, [16, 4000])]
+    wants = [s.eager()[0] for s in steps]
+    torch.cuda.synchronize()
+    turn, failed = threading.Barrier(2, timeout=60), []
+
+    def work(s, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    s.reset()
+                    for i in range(len(want)):
+                        s.feed(i)
+                        turn.wait()
+                        if not same(s.run(), want[i]):
+                            failed.append(i)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:
+            failed.append(e)
+            turn.abort()
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(steps, wants)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(100)
+    assert not failed, failed
