@@ -497,7 +497,8 @@ typedef struct {
  *   i < R/2, R = rotary_dim, turn by positions[t] * inv_freq[i] (the angle
  *   formed and reduced in 64 bits): (a cos - b sin, b cos + a sin);
  *   y[R..] stays.
- * R is a multiple of 8 from 0 to head_dim.  All device arrays, on 4 bytes. */
+ * R is a multiple of 8 from 0 to head_dim; fewer than 2^24 tokens a call.  All
+ * device arrays, on 4 bytes. */
 typedef struct {
   const float* q_scale;              /* [head_dim] or NULL: no norm of q */
   const float* k_scale;              /* [head_dim] or NULL: no norm of k */

@@ -109,6 +109,9 @@ bool rows_clash(const rtenhip_tensor* a, const rtenhip_tensor* b);
 // (what is written must not be written twice).
 bool rows_apart(const int64_t* n, const int64_t* strides, int count, int64_t dim);
 
+// A launch has fewer than 2^32 threads.
+inline bool launchable(int64_t blocks, int64_t threads) { return blocks * threads <= int64_t(UINT32_MAX); }
+
 // Makes the context's device current for a launch and puts back the caller's.
 struct DeviceScope {
   int before = -1;

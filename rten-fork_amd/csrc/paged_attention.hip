@@ -1610,7 +1610,7 @@ static rtenhip_status paged_plan(const rtenhip_tensor* q, const rtenhip_kv_cache
     d.target_big = PA_TARGET_BIG;
     if (small) p.grid_small = small_tiles + (splits ? d.target_small : 0);
     if (big) p.grid_big = big_tiles + (splits ? d.target_big : 0);
-    if (p.grid_small > INT32_MAX || p.grid_big > INT32_MAX)
+    if (!launchable(p.grid_small, PA_THREADS) || !launchable(p.grid_big, 2 * d.rows_big))
       return fail(RTENHIP_UNSUPPORTED_VALUE, "Too many query rows");
     if (splits) {
       p.slots_small = small ? d.target_small * 3 / 2 : 0;

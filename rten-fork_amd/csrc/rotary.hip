@@ -345,6 +345,7 @@ static rtenhip_status rotary_desc(const rtenhip_tensor* q, const rtenhip_tensor*
   if (tokens < 0 || tokens > INT32_MAX || q->shape[1] < 0 || q->shape[1] > 65536 || k->shape[1] < 0 ||
       k->shape[1] > 65536)
     return fail(RTENHIP_INVALID_VALUE, "Invalid input size");
+  if (!launchable(tokens, ROT_THREADS)) return fail(RTENHIP_UNSUPPORTED_VALUE, "Too many tokens");
   if (r->rotary_dim < 0 || r->rotary_dim > dim || r->rotary_dim % 8)
     return fail(RTENHIP_UNSUPPORTED_VALUE, "rotary_dim must be a multiple of 8 up to head_dim");
   if (!(r->epsilon >= 0.f)) return fail(RTENHIP_INVALID_VALUE, "epsilon must not be negative");

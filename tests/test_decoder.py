@@ -217,6 +217,22 @@ def test_append(d):
         assert st == code and text in msg, (kw, st, msg)
 
 
+def test_more_workgroups_than_a_launch_has(d):
+    """A launch has fewer than 2^32 threads."""
+    n = (1 << 24) - 1
+    assert rot(d, q=tensor(d, 0, n, 1, 8), k=tensor(d, 100, n, 1, 8), qo=tensor(d, 200, n, 1, 8), ko=tensor(d, 300, n, 1, 8),
+               r=rotary(d, rotary_dim=8)) == (MISSING, "Missing context")
+    n += 1
+    assert rot(d, q=tensor(d, 0, n, 1, 8), k=tensor(d, 100, n, 1, 8), qo=tensor(d, 200, n, 1, 8), ko=tensor(d, 300, n, 1, 8),
+               r=rotary(d, rotary_dim=8)) == (UNSUPPORTED, "Too many tokens")
+    c, s = cache(d, heads=64, dim=8), seqs(d, 1 << 18, pages=1, starts=False)
+    st, msg = attention(d, q=tensor(d, 0, 1 << 18, 64, 8), c=c, s=s, out=tensor(d, 100, 1 << 18, 64, 8))
+    assert st == UNSUPPORTED and "Too many query rows" in msg
+    s = seqs(d, (1 << 18) - 1, pages=1, starts=False)
+    assert attention(d, q=tensor(d, 0, (1 << 18) - 1, 64, 8), c=c, s=s,
+                     out=tensor(d, 100, (1 << 18) - 1, 64, 8)) == (MISSING, "Missing context")
+
+
 def test_sample(d):
     def samp(x=None, f=None, u=BASE + 5 * GIB, ws=BASE + 6 * GIB, n=1 << 40, tokens=BASE + 7 * GIB, lp=None):
         return call(d, "rtenhip_sample_f32", None, C.byref(x or tensor(d, 0, 3, 1000)),
