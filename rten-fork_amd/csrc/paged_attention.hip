@@ -186,7 +186,6 @@ __device__ bool plan(const PagedDesc& d, int block, PlanShared& sh, Work& out) {
     // (More pieces than workgroups: q_starts do not rise, and some stretches
     // never come.  Nothing is joined then.)
     d.slots[BIG] = all > (int)gridDim.x ? 0 : min(n, BIG ? d.slots_big : d.slots_small);
-    if (!(BIG ? d.grid_small : d.grid_big)) d.slots[!BIG] = 0;  // the other kernel does not run
   }
   int at = items_in - items, slot = slots_in - slots;
   for (int w = 0; w < wave; w++) at += sh.items[w], slot += sh.slots[w];
