@@ -165,24 +165,27 @@ __device__ __forceinline__ int find_seq(const SeqView& v, int t) {
   }
 }
 
-// cos and sin of pos * f.  The angle is formed and brought within a quarter
-// of pi in 64 bits (at position 10^6 its error is 10^-10; in 32 bits it would
-// be 0.06), the rest are the Taylor series of sin and cos in 32 bits: the
-// first terms left out, x^11 / 11! and x^12 / 12!, are below 2^-29 there.
+// cos and sin of pos * f, rounded once.  The angle is formed and brought within
+// a quarter of pi in 64 bits (at position 10^6 its error is 10^-10; in 32 bits
+// it would be 0.06), and so are the Taylor series of sin and cos: the first
+// terms left out, x^13 / 13! and x^14 / 14!, are below 2^-36 there.
 __device__ __forceinline__ void turn_of(double pos, float f, float& c, float& s) {
   const double angle = pos * (double)f;
   const double n = __builtin_rint(angle * 0.63661977236758134308);
   double r = __builtin_fma(-n, 1.57079632679489655800, angle);
   r = __builtin_fma(-n, 6.12323399573676603587e-17, r);
-  const float x = (float)r, x2 = x * x;
-  float ps = __fmaf_rn(x2, 2.7557319e-6f, -1.9841270e-4f);
-  ps = __fmaf_rn(x2, ps, 8.3333333e-3f);
-  ps = __fmaf_rn(x2, ps, -1.6666667e-1f);
-  const float sn = __fmaf_rn(x * x2, ps, x);
-  float pc = __fmaf_rn(x2, -2.7557319e-7f, 2.4801587e-5f);
-  pc = __fmaf_rn(x2, pc, -1.3888889e-3f);
-  pc = __fmaf_rn(x2, pc, 4.1666667e-2f);
-  const float cs = __fmaf_rn(x2 * x2, pc, __fmaf_rn(x2, -0.5f, 1.0f));
+  const double x2 = r * r;
+  double ps = __builtin_fma(x2, -1. / 39916800., 1. / 362880.);
+  ps = __builtin_fma(x2, ps, -1. / 5040.);
+  ps = __builtin_fma(x2, ps, 1. / 120.);
+  ps = __builtin_fma(x2, ps, -1. / 6.);
+  const float sn = (float)__builtin_fma(r * x2, ps, r);
+  double pc = __builtin_fma(x2, 1. / 479001600., -1. / 3628800.);
+  pc = __builtin_fma(x2, pc, 1. / 40320.);
+  pc = __builtin_fma(x2, pc, -1. / 720.);
+  pc = __builtin_fma(x2, pc, 1. / 24.);
+  pc = __builtin_fma(x2, pc, -1. / 2.);
+  const float cs = (float)__builtin_fma(x2, pc, 1.);
   const int q = (int)(long long)n & 3;
   const float a = q & 1 ? sn : cs, b = q & 1 ? cs : sn;
   c = (q == 1 || q == 2) ? -a : a;
@@ -211,7 +214,9 @@ constexpr int ROT_AHEAD = 4;  // rows a lane has in flight
 
 // One token per workgroup (blockIdx.x); LPR lanes per head row, each with the
 // 8 elements of four pairs, so a row needs no exchange but the sum of its
-// squares, and a lane's four turns are formed once and used for all its rows.
+// squares.  The token's turns are formed once, one by a thread, and shared
+// through LDS (8192 tokens of 4 + 2 heads of 128 take 15.3 us, and 17.5 where
+// each lane forms its four, in 32 bits).
 // gridDim.y workgroups share a token's rows where there are few tokens.
 // Bound by memory: rows are read once and written once.  8192 tokens of 32 + 8
 // heads of 128 into a bf16 cache: 72 us, 5.1 TB/s (a copy of 4 GiB: 4.7); one
@@ -219,6 +224,7 @@ constexpr int ROT_AHEAD = 4;  // rows a lane has in flight
 template <int LPR, int TYPE, bool APPEND, bool INTER>
 __global__ __launch_bounds__(ROT_THREADS) void rotary_kernel(RotaryDesc d) {
   constexpr int RPP = ROT_THREADS / LPR;  // rows per pass of the workgroup
+  __shared__ __attribute__((aligned(16))) float cos_sh[ROT_THREADS / 2], sin_sh[ROT_THREADS / 2];
   const int t = blockIdx.x;
   const int j = threadIdx.x % LPR, sub = threadIdx.x / LPR;
   const bool live = j * 8 < d.dim, turned = j * 8 < d.rot;
@@ -238,12 +244,17 @@ __global__ __launch_bounds__(ROT_THREADS) void rotary_kernel(RotaryDesc d) {
     }
   }
   if (d.positions) pos = d.positions[t];
-  float cs[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {0.f, 0.f, 0.f, 0.f};
-  if (turned) {
-    const float* f = d.inv_freq + 4 * j;
-#pragma unroll
-    for (int i = 0; i < 4; i++) turn_of((double)pos, f[i], cs[i], sn[i]);
+  float4 cs4 = make_float4(1.f, 1.f, 1.f, 1.f), sn4 = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (d.rot) {
+    if ((int)threadIdx.x < d.rot / 2) {
+      float c, s;
+      turn_of((double)pos, d.inv_freq[threadIdx.x], c, s);
+      cos_sh[threadIdx.x] = c, sin_sh[threadIdx.x] = s;
+    }
+    __syncthreads();  // (padding has left as a whole)
+    if (turned) cs4 = *(const float4*)&cos_sh[4 * j], sn4 = *(const float4*)&sin_sh[4 * j];
   }
+  const float cs[4] = {cs4.x, cs4.y, cs4.z, cs4.w}, sn[4] = {sn4.x, sn4.y, sn4.z, sn4.w};
 
   for (int r0 = (blockIdx.y * RPP) + sub; r0 < d.rows; r0 += gridDim.y * RPP * ROT_AHEAD) {
     float x[ROT_AHEAD][8];

@@ -1125,3 +1125,25 @@ def test_decoder_threads(rh):
     for t in threads:
         t.join(100)
     assert not failed, failed
+
+
+@pytest.mark.parametrize("inter", [False, True])
+def test_rotary_turns_are_rounded_once(rh, inter):
+    """Pairs (1, 0) turn into cos and sin, off by half a step of float32."""
+    import torch
+
+    pos = torch.cat([torch.arange(300), torch.randint(0, 1_000_000, (300,), generator=torch.Generator().manual_seed(1))]).int()
+    half = 64
+    freq = (10000.0 ** (-torch.arange(half).double() / half)).float()
+    x = torch.zeros(len(pos), 1, 2 * half)
+    x[..., 0::2] = 1
+    if not inter:
+        x = torch.cat((torch.ones(len(pos), 1, half), torch.zeros(len(pos), 1, half)), -1)
+    got = rh.qk_norm_rotary(x.cuda(), x.cuda(), pos.cuda(), freq.cuda(), interleaved=inter)[0].cpu().numpy()[:, 0]
+    a = pos.numpy().astype(np.float64)[:, None] * freq.numpy().astype(np.float64)
+    for part, want in ((slice(0, None, 2) if inter else slice(0, half), np.cos(a)),
+                       (slice(1, None, 2) if inter else slice(half, None), np.sin(a))):
+        # (2^-36 of the series left out beside half a step, 2^-25 at least of a
+        # number above 1/2; smaller cosines and sines come from smaller x.)
+        step = np.spacing(np.abs(want).astype(np.float32)).astype(np.float64)
+        assert (np.abs(got[:, part] - want) <= step * (0.5 + 2.0 ** -10)).all()
