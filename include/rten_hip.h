@@ -534,8 +534,13 @@ rtenhip_status rtenhip_qk_norm_rotary_append_f32(rtenhip_ctx* ctx, const rtenhip
  * if 0 <= j <= p, j has a page, and window == 0, or j > p - window, or
  * j < sinks:
  *   out = sum_j softmax_j(scale * q . k_j) v_j,  zeros if it sees none.
- * Products of a 16-bit or f32 cache are formed to about 22 bits and summed in
- * 32.  Slots that no query of the call sees are read but have no effect,
+ * Products are formed to about 22 bits and summed in 32: a number of q, of the
+ * cache or of the weights counts with an error of at most 2^-22 of itself or
+ * 2^-26 of the largest of its row of head_dim (of a weight: 2^-23 of the row's
+ * largest).  A token's size does not matter to queries that do not see it
+ * (beside values above 2^53 those below 2^-94 may vanish).  Sums overflow where
+ * values times the number of tokens that count pass the range of 32 bits.
+ * Slots that no query of the call sees are read but have no effect,
  * whatever they hold; a NaN or an infinity in a key or value leaves the
  * queries that do not see its token as they are (the output of those that do
  * is undefined).  out may be q.  workspace: at least

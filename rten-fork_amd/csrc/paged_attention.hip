@@ -344,9 +344,10 @@ struct CacheType {
 // terms (exact products, 22 bits of q and p), bf16 into three bf16 terms.
 // Bound by the cache's bytes: DEPTH tiles are on their way in registers while
 // one is worked on.  64 ragged sequences of 60 to 6000 keys (f16, 8 heads of
-// 128, 0.80 GB): 163 us, 4.9 TB/s; 131,072 keys of one sequence (f32, 1.07 GB):
-// 183 us, 5.9 TB/s; 32 windows of 4096 (bf16, 8 heads of 64, 0.27 GB): 64 us,
-// 4.2 TB/s.  A copy of 4 GiB runs at 4.7.
+// 128, 0.80 GB): 160 us, 5.0 TB/s; 131,072 keys of one sequence (f32, 1.07 GB):
+// 188 us with the join, 5.7 TB/s; 32 windows of 4096 (bf16, 8 heads of 64, 0.27
+// GB): 64 us, 4.2 TB/s.  A copy of 4 GiB runs at 4.7.  The matrix instructions
+// are busy for 9, 27 and 11 % of the time.
 template <int DP, int TYPE>
 struct DecodeTile {
   static constexpr int DPL = DP / 16;                                // value dimensions of a lane
@@ -357,7 +358,8 @@ struct DecodeTile {
   // us; of f32 rows, twice as long, one is enough: 188 against 208 us over
   // 131,072 keys, where two leave no registers.  Windows of bf16 rows of 64:
   // 64 us with 3 waves, 63 with 2 and 67 with 4; ragged sequences of them 104,
-  // 110 and 110.)
+  // 110 and 110.  f32 rows of 256, 64 ragged sequences: 684 us with one wave,
+  // 1206 with two, which spill; 16-bit rows would take two, f16 308 us for 341.)
   static constexpr int WAVES = DP == 64 ? 3 : DP == 128 ? 2 : 1;
   static constexpr int DEPTH = DP == 64 || (DP == 128 && TYPE != RTENHIP_CACHE_F32) ? 2 : 1;
   static constexpr int QW = TYPE == RTENHIP_CACHE_F32 ? DP / 4 : TYPE == RTENHIP_CACHE_F16 ? DP / 4 : 3 * DP / 8;
@@ -810,10 +812,13 @@ __global__ __launch_bounds__(PA_THREADS, (DecodeTile<DP, TYPE>::WAVES)) void dec
 // it multiplies and the other after, which keeps one's conversions and
 // exponentials under the other's products; at head_dim 256 a wave needs all of
 // a SIMD's registers, and four waves work on tiles of 32 keys.
-// Bound by the matrix instructions at long prompts: 8192 tokens of 32 heads of
-// 128 on an f32 cache, 550 GFLOP and three f16 products for each, 1.65 ms, 1.0
-// PFLOP/s of them (a library's f16 product of 8192^3: 1.19; f32 instructions
-// alone would take 3.6 ms).
+// Bound by the matrix instructions, and what has to be converted between them,
+// at long prompts: 8192 tokens of 32 heads of 128 on an f32 cache, 550 GFLOP and
+// three f16 products for each, 1.6 ms, 1.0 PFLOP/s of them (a library's f16
+// product of 8192^3: 1.19; f32 instructions alone would take 3.6 ms).  Matrix
+// instructions run for 49 % of the SIMDs' cycles, vector ones issue for 51 %.
+// 4096 tokens on a bf16 cache 0.32 ms, on f16 0.29; 2048 tokens of 16 heads of
+// 256, f32, 0.30 ms.
 template <int DP, int TYPE>
 struct ChunkTile {
   static constexpr int WAVES = DP == 256 ? 4 : 8, THREADS = 64 * WAVES;

@@ -219,8 +219,8 @@ constexpr int ROT_AHEAD = 4;  // rows a lane has in flight
 // each lane forms its four, in 32 bits).
 // gridDim.y workgroups share a token's rows where there are few tokens.
 // Bound by memory: rows are read once and written once.  8192 tokens of 32 + 8
-// heads of 128 into a bf16 cache: 72 us, 5.1 TB/s (a copy of 4 GiB: 4.7); one
-// token 3 us, a launch.
+// heads of 128 into a bf16 cache, 369 MB: 71.5 us, 5.2 TB/s (a copy of 4 GiB:
+// 4.7); one token 3.2 us, a launch.
 template <int LPR, int TYPE, bool APPEND, bool INTER>
 __global__ __launch_bounds__(ROT_THREADS) void rotary_kernel(RotaryDesc d) {
   constexpr int RPP = ROT_THREADS / LPR;  // rows per pass of the workgroup
@@ -329,9 +329,9 @@ static rtenhip_status launch_rotary(const RotaryDesc& d, int64_t tokens, hipStre
   const int rpp = ROT_THREADS / lpr;
   // Few tokens: a workgroup per pass of a token's rows, so that no load waits
   // for another; many tokens fill the card by themselves and then share the
-  // turns among all rows.  (32 + 8 heads of 128: one token 3.6 against 5.3 us
-  // with one workgroup, 400 tokens 6.2 and 6.3, 1024 10.7 and 10.3, 8192 79 and
-  // 73.)
+  // turns among all rows.  (32 + 8 heads of 128: one token 3.2 against 4.4 us
+  // with one workgroup, 400 tokens 5.9 and 6.2, 1024 10.3 and 10.1, 8192 74 and
+  // 71.5.)
   const int passes = (d.rows + rpp - 1) / rpp;
   const dim3 grid((unsigned)tokens, (unsigned)(tokens < 512 ? passes : 1));
   if (lpr == 8)
