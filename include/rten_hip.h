@@ -538,7 +538,7 @@ rtenhip_status rtenhip_qk_norm_rotary_append_f32(rtenhip_ctx* ctx, const rtenhip
  * cache or of the weights counts with an error of at most 2^-22 of itself or
  * 2^-26 of the largest of its row of head_dim (of a weight: 2^-23 of the row's
  * largest).  A token's size does not matter to queries that do not see it
- * (beside values above 2^53 those below 2^-94 may vanish).  Sums overflow where
+ * (beside values above 2^53 those below 2^-93 lose bits).  Sums overflow where
  * values times the number of tokens that count pass the range of 32 bits.
  * Slots that no query of the call sees are read but have no effect,
  * whatever they hold; a NaN or an infinity in a key or value leaves the

@@ -796,7 +796,7 @@ __global__ __launch_bounds__(PA_THREADS, (DecodeTile<DP, TYPE>::WAVES)) void dec
 //    computed again with a power of two for each key and each value's row, and
 //    the products of values of different loudness apart (careful).  Up to there
 //    a row is exact to 2^-26 of its own largest number and p to 2^-23 of the
-//    largest p, finer than the split's 22 bits.  (Values below 2^-94 can vanish
+//    largest p, finer than the split's 22 bits.  (Values below 2^-93 lose bits
 //    beside others above 2^53 in either pass.)
 //  - S^T = K Q^T: a lane (n, h) has row n's scores for the keys
 //    8 i + 4 h + j of each 32, so the softmax needs one exchange with lane
@@ -889,8 +889,8 @@ struct __attribute__((aligned(16))) TileInfo {
 
 // How many binades the largest numbers of 8 keys may lie apart to share an
 // exponent, how many the values of a tile below the result's scale, and that
-// scale's least exponent (no sum of 2^127s that counts overflows, and there are
-// 85 binades below 1).
+// scale's least exponent (2^27 values of 2^127 can be added, and there are 85
+// binades below 1).
 constexpr uint32_t EVEN = 12;
 constexpr int FALL = 10, O_LEAST = -41;
 constexpr int NO_VALUE = 127;  // the exponent of values that are all zero (or below 2^-133)

@@ -1147,3 +1147,23 @@ def test_rotary_turns_are_rounded_once(rh, inter):
         # number above 1/2; smaller cosines and sines come from smaller x.)
         step = np.spacing(np.abs(want).astype(np.float32)).astype(np.float64)
         assert (np.abs(got[:, part] - want) <= step * (0.5 + 2.0 ** -10)).all()
+
+
+def test_thread_ends_before_its_work(rh):
+    """A thread's context goes with it; what it queued is still done."""
+    import threading
+
+    import torch
+
+    x, w = torch.randn(2048, 2048).cuda(), torch.randn(2048, 2048).cuda()
+    want, got = rh.matmul(x, w), []
+
+    def work():
+        got.append([rh.matmul(x, w) for _ in range(20)][-1])
+
+    for _ in range(3):
+        t = threading.Thread(target=work)
+        t.start()
+        t.join(60)
+    torch.cuda.synchronize()
+    assert len(got) == 3 and all(torch.equal(y, want) for y in got)
